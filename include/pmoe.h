@@ -37,6 +37,9 @@ enum {
 
 enum { PMOE_SCORE_SOFTMAX = 0, PMOE_SCORE_SIGMOID = 1 };
 
+/* Element types of arrays that come in more than one. */
+enum { PMOE_F32 = 0, PMOE_BF16 = 1, PMOE_F16 = 2 };
+
 /* Component order inside one slab slot (names as slab.py:90-126 keys). */
 enum {
   PMOE_GATE_W = 0, PMOE_GATE_S, PMOE_GATE_B,
@@ -50,12 +53,19 @@ enum {
  * [inter, hidden/group]; down weight u32 [hidden, inter*bits/32],
  * scales/biases bf16 [hidden, inter/group] (safetensors_index.py:8-25,
  * bench/slab_probe.py:82).  off[c] is the byte offset of component c inside a
- * slot, expert_bytes the slot stride. */
+ * slot, expert_bytes the slot stride.
+ *
+ * bits 4 with group 32 is the microscaled format (pmoe_mx4_quantize): scales
+ * are u8 [.., cols/32] and the biases components are empty.  Dims are
+ * multiples of 32, and the slab, expert_bytes and the weight components'
+ * offsets multiples of 16 bytes.  Every entry point that takes a geometry takes
+ * either format.  A row whose activations hold an infinity or a NaN, or whose
+ * intermediate leaves fp32, comes out as NaN there. */
 typedef struct {
   int32_t hidden;
   int32_t inter;
   int32_t bits;   /* 4 or 6 */
-  int32_t group;  /* 64 */
+  int32_t group;  /* 64; 32: microscaled 4-bit */
   int64_t expert_bytes;
   int64_t off[PMOE_NCOMP];
   int64_t nbytes[PMOE_NCOMP];
@@ -135,6 +145,22 @@ int pmoe_quantize(const float* w, int rows, int cols, int bits, int group,
 int pmoe_dequant(const uint32_t* q, const uint16_t* scales,
                  const uint16_t* biases, int rows, int cols, int bits,
                  int group, uint16_t* out, void* stream);
+
+/* Microscaled 4-bit format (MX: E2M1 elements, E8M0 scales; mlx's "mxfp4"
+ * mode): w [rows, cols] of a PMOE_F32 / BF16 / F16 dtype -> q u32 [rows,
+ * cols / 8] and one scale for each 32 values, u8 [rows, cols / 32], a power of
+ * two biased by 127: 2^(floor(log2 max|w|) - 2), no less than 2^-127.  A code
+ * is 1 sign, 2 exponent and 1 mantissa bit, +-{0, 0.5, 1, 1.5, 2, 3, 4, 6}, to
+ * nearest with ties to the even mantissa and above 6 to 6.  A group that holds
+ * an infinity or a NaN gets scale 255: all its values read back as NaN.  cols:
+ * a multiple of 32. */
+int pmoe_mx4_quantize(const void* w, int dtype, int rows, int cols, uint32_t* q,
+                      uint8_t* scales, void* stream);
+
+/* The values that such codes stand for, rounded once to dtype (exact but
+ * where they leave its range). */
+int pmoe_mx4_dequant(const uint32_t* q, const uint8_t* scales, int rows, int cols, int dtype,
+                     void* out, void* stream);
 
 /* ---- expert compute --------------------------------------------------- */
 

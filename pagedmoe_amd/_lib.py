@@ -22,6 +22,7 @@ COMPONENTS = (
 )
 SCORE_SOFTMAX = 0
 SCORE_SIGMOID = 1
+F32, BF16, F16 = 0, 1, 2
 
 
 class PmoeError(RuntimeError):
@@ -83,6 +84,8 @@ SIGNATURES = {
     "pmoe_dispatch": (_I, [_P, _I, _I, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     "pmoe_quantize": (_I, [_P, _I, _I, _I, _I, _P, _P, _P, _P]),
     "pmoe_dequant": (_I, [_P, _P, _P, _I, _I, _I, _I, _P, _P]),
+    "pmoe_mx4_quantize": (_I, [_P, _I, _I, _I, _P, _P, _P]),
+    "pmoe_mx4_dequant": (_I, [_P, _P, _I, _I, _I, _P, _P]),
     "pmoe_moe_workspace": (_SZ, [ctypes.POINTER(Geom), _I, _I, _I, _I]),
     "pmoe_moe_workspace_init": (_I, [_P, _SZ, _P]),
     "pmoe_moe_workspace_status": (_I, [_P, ctypes.POINTER(ctypes.c_uint32), _P]),
@@ -187,6 +190,11 @@ def check(rc: int, what: str = "") -> None:
     if rc != PMOE_OK:
         msg = lib().pmoe_last_error().decode(errors="replace")
         raise PmoeError(f"{what or 'pmoe'} failed ({rc}): {msg}")
+
+
+def is_mx(g: Geom) -> bool:
+    """Whether a geometry's experts are in the microscaled 4-bit format."""
+    return g.group == 32
 
 
 def geom(hidden: int, inter: int, bits: int, group: int = 64) -> Geom:

@@ -40,12 +40,13 @@ class HostExpertStore:
         self.bytes = np.frombuffer(buf, dtype=np.uint8)
 
     @classmethod
-    def from_checkpoint(cls, model_dir, layers=None, group: int = 64) -> "HostExpertStore":
+    def from_checkpoint(cls, model_dir, layers=None, group: int | None = None) -> "HostExpertStore":
         """A store holding every expert of the MoE layers of a quantized
         safetensors checkpoint (stacked or per-expert layout), read straight
         from the files into slot layout (checkpoint.py).  ``layers`` keeps
         only those layer numbers; ``layer_numbers`` lists the store's layers
-        in order."""
+        in order.  ``group`` is the format's group size: by default what the
+        scales say, 32 (microscaled 4-bit) where they are U8, else 64."""
         from . import checkpoint as ck
         from ._lib import geom
 
@@ -57,6 +58,8 @@ class HostExpertStore:
         if not found:
             raise PmoeError(f"{model_dir}: no quantized MoE expert tensors found")
         layouts = [ck.layer_layout(path, index) for _, path in found]
+        if group is None:
+            group = 32 if layouts[0].microscaled else 64
         hidden, inter, bits = layouts[0].geometry(group)
         g = geom(hidden, inter, bits, group)
         store = cls(g, len(layouts), layouts[0].n_experts)

@@ -17,6 +17,10 @@ gate/up/down weight, scales, biases) -- no conversion, the checkpoint on disk
 stays as it is.  The u32 weight words and bf16 scale/bias rows are the
 layout the kernels read (row-major per expert), so the bytes are copied
 unchanged.
+
+A checkpoint in the microscaled 4-bit format (mlx's "mxfp4" mode) has no biases
+and scales of U8, one for 32 values; its experts are read with six ``pread``
+calls into a group-32 geometry.
 """
 
 from __future__ import annotations
@@ -29,7 +33,7 @@ from pathlib import Path
 
 import numpy as np
 
-from ._lib import COMPONENTS, Geom, PmoeError
+from ._lib import COMPONENTS, Geom, PmoeError, is_mx
 
 _ITEMSIZE = {"F64": 8, "F32": 4, "F16": 2, "BF16": 2, "I64": 8, "I32": 4, "I16": 2,
              "I8": 1, "U8": 1, "U32": 4, "U16": 2, "BOOL": 1}
@@ -127,7 +131,7 @@ def read_headers(model_dir) -> dict:
 
 
 class ExpertLayout:
-    """The nine components of one MoE layer: component name
+    """The nine components (microscaled: six) of one MoE layer: component name
     ("gate_proj.weight" ...) -> a stacked TensorLoc or {expert: TensorLoc}."""
 
     def __init__(self, path: str, parts: dict):
@@ -150,6 +154,11 @@ class ExpertLayout:
         if e not in v:
             raise KeyError(f"{self.path}: no tensor for expert {e} of {name}")
         return v[e]
+
+    @property
+    def microscaled(self) -> bool:
+        """U8 scales: the microscaled 4-bit format."""
+        return self.loc("gate_proj.scales", 0).dtype == "U8"
 
     def geometry(self, group: int = 64):
         """(hidden, inter, bits) from the gate projection's shapes:
@@ -183,6 +192,11 @@ def layer_layout(path: str, index: dict) -> ExpertLayout:
             if m and m.group(2) in _PROJS:
                 parts.setdefault(f"{m.group(2)}.{m.group(3)}", {})[int(m.group(1))] = loc
     missing = [c for c in COMPONENTS if c not in parts]
+    if missing and all(c.endswith(".biases") for c in missing) and len(missing) == 3:
+        scales = parts["gate_proj.scales"]
+        first = scales if isinstance(scales, TensorLoc) else next(iter(scales.values()))
+        if first.dtype == "U8":  # microscaled: no biases
+            missing = []
     if missing:
         raise KeyError(f"{path}: checkpoint lacks {missing} (quantized experts with scales "
                        "and biases are required)")
@@ -209,9 +223,13 @@ def check_layout(layout: ExpertLayout, g: Geom) -> None:
     from .slab import component_specs
 
     specs = component_specs(g)
-    want_dtype = {"weight": ("U32", "I32"), "scales": ("BF16",), "biases": ("BF16",)}
-    for c, name in enumerate(COMPONENTS):
-        shape, _, nbytes, _ = specs[name]
+    want_dtype = {"weight": ("U32", "I32"), "scales": ("U8",) if is_mx(g) else ("BF16",),
+                  "biases": ("BF16",)}
+    if is_mx(g) != layout.microscaled:
+        raise PmoeError(f"{layout.path}: the checkpoint's scales are "
+                        f"{layout.loc('gate_proj.scales', 0).dtype}; the slab holds "
+                        f"{'/'.join(want_dtype['scales'])}")
+    for name, (shape, _, nbytes, _) in specs.items():
         kind = name.split(".")[1]
         for e in range(layout.n_experts):
             loc = layout.loc(name, e)
@@ -248,7 +266,7 @@ class _Files:
 
 
 def read_expert(layout: ExpertLayout, e: int, g: Geom, out: np.ndarray, files=None) -> None:
-    """Expert e's nine byte ranges into ``out`` (uint8, one slot:
+    """Expert e's byte ranges (nine; six microscaled) into ``out`` (uint8, one slot:
     ``g.expert_bytes``) at the slot's component offsets."""
     if out.dtype != np.uint8 or out.size != int(g.expert_bytes):
         raise ValueError(f"out must be {int(g.expert_bytes)} uint8, got {out.size} {out.dtype}")
@@ -257,6 +275,8 @@ def read_expert(layout: ExpertLayout, e: int, g: Geom, out: np.ndarray, files=No
     try:
         for c, name in enumerate(COMPONENTS):
             off, nb = int(g.off[c]), int(g.nbytes[c])
+            if nb == 0:
+                continue
             loc = layout.loc(name, e)
             if loc.nbytes != nb:
                 raise PmoeError(f"{layout.path}: {name} of expert {e} is {loc.nbytes} B, the "

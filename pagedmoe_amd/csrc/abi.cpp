@@ -36,7 +36,8 @@ Profiler& prof() {
 
 const char* kNames[K_COUNT] = {"router_logits", "route_select", "dispatch",  "qgemv_gateup",
                                "qgemv_down",    "combine",      "prefill_gateup", "prefill_down",
-                               "decode_fused",  "decode_xcd",   "experts_xcd"};
+                               "decode_fused",  "decode_xcd",   "experts_xcd",    "mx_split",
+                               "mx_gateup",     "mx_down",      "block_norm"};
 
 }  // namespace
 
@@ -119,18 +120,23 @@ extern "C" int pmoe_geom_init(pmoe_geom* g, int hidden, int inter, int bits, int
   pmoe::clear_error();
   if (!g) return pmoe::fail(PMOE_EINVAL, "geom_init: null pointer");
   if (bits != 4 && bits != 6) return pmoe::fail(PMOE_EINVAL, "geom_init: bits must be 4 or 6");
-  if (group != 64) return pmoe::fail(PMOE_EINVAL, "geom_init: group must be 64");
-  if (hidden <= 0 || inter <= 0 || hidden % 64 || inter % 64)
-    return pmoe::fail(PMOE_EINVAL, "geom_init: hidden and inter must be positive multiples of 64");
+  const bool mx = group == 32;  // microscaled 4-bit: u8 scales, no biases
+  if (mx ? bits != 4 : group != 64)
+    return pmoe::fail(PMOE_EINVAL, "geom_init: group must be 64, or 32 with 4 bits (microscaled)");
+  if (hidden <= 0 || inter <= 0 || hidden % group || inter % group)
+    return pmoe::fail(PMOE_EINVAL, "geom_init: hidden and inter must be positive multiples of " +
+                                       std::to_string(group));
   g->hidden = hidden;
   g->inter = inter;
   g->bits = bits;
   g->group = group;
   const int64_t up_w = int64_t(inter) * (int64_t(hidden) * bits / 32) * 4;
-  const int64_t up_s = int64_t(inter) * (hidden / group) * 2;
+  const int item = mx ? 1 : 2;
+  const int64_t up_s = int64_t(inter) * (hidden / group) * item;
   const int64_t dn_w = int64_t(hidden) * (int64_t(inter) * bits / 32) * 4;
-  const int64_t dn_s = int64_t(hidden) * (inter / group) * 2;
-  const int64_t sizes[PMOE_NCOMP] = {up_w, up_s, up_s, up_w, up_s, up_s, dn_w, dn_s, dn_s};
+  const int64_t dn_s = int64_t(hidden) * (inter / group) * item;
+  const int64_t up_b = mx ? 0 : up_s, dn_b = mx ? 0 : dn_s;
+  const int64_t sizes[PMOE_NCOMP] = {up_w, up_s, up_b, up_w, up_s, up_b, dn_w, dn_s, dn_b};
   int64_t off = 0;
   for (int c = 0; c < PMOE_NCOMP; ++c) {
     g->off[c] = off;

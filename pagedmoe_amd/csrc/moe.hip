@@ -6,9 +6,12 @@
 // shared-expert add (restated tests/test_stream.py:198).  The combine is a
 // fixed-order fp32 reduction: out[n] = fma over k = 0..K-1 of w[n,k]*y[n,k],
 // then the shared expert, so results do not depend on scheduling.
+#include <algorithm>
 #include <mutex>
 #include <string>
 
+#include "mx_experts.h"
+#include "mx_pieces.h"
 #include "pmoe_internal.h"
 #include "pmoe_kernels.h"
 #include "route_common.h"
@@ -45,6 +48,11 @@ struct MoeWs {
   size_t dws_bytes = 0;
   void* record = nullptr;         // decode routing record
   int max_tiles = 0;
+  // microscaled experts: the tokens' activation pieces, scales and step masks,
+  // the sorted rows' intermediate (mx_experts.h)
+  uint8_t *xpair = nullptr, *xthird = nullptr, *xscale = nullptr;
+  uint16_t* xsteps = nullptr;
+  uint8_t *hpair = nullptr, *hscale = nullptr;
 };
 
 struct Carver {
@@ -75,11 +83,23 @@ size_t carve(const pmoe_geom* g, int n, int k, int shared, int n_experts, void* 
   t.active = c.take<int32_t>(n_ids);
   t.n_active = c.take<int32_t>(1);
   // tile capacity for the shortest prefill tiles
-  t.max_tiles = int(rows / prefill_min_tile_rows()) + n_ids + 1;
+  const bool mx = is_mx(g);
+  t.max_tiles = int(rows / (mx ? mx_min_tile_rows() : prefill_min_tile_rows())) + n_ids + 1;
   t.tiles = c.take<int4>(t.max_tiles);
   t.n_tiles = c.take<int32_t>(1);
-  t.h = c.take<uint16_t>(rows * g->inter);
-  t.y = c.take<float>(rows * g->hidden);
+  if (mx) {
+    const size_t xg = size_t(n) * (g->hidden / kMxGroup), hg = rows * (g->inter / kMxGroup);
+    t.xpair = c.take<uint8_t>(xg * kMxPairBytes);
+    t.xthird = c.take<uint8_t>(xg * kMxThirdBytes);
+    t.xscale = c.take<uint8_t>(xg);
+    t.xsteps = c.take<uint16_t>(size_t(n) * 4);
+    t.hpair = c.take<uint8_t>(hg * kMxPairBytes);
+    t.hscale = c.take<uint8_t>(hg);
+    t.y = reinterpret_cast<float*>(c.take<uint16_t>(rows * g->hidden));  // bf16 rows only
+  } else {
+    t.h = c.take<uint16_t>(rows * g->inter);
+    t.y = c.take<float>(rows * g->hidden);
+  }
   t.dws_bytes = dispatch_workspace(int(rows), n_ids);
   t.dws = c.take<uint8_t>(t.dws_bytes);
   t.record = c.take<uint8_t>(decode_record_bytes());
@@ -184,9 +204,19 @@ __global__ __launch_bounds__(256) void zero_dropped_rows_kernel(const int32_t* _
   for (int i = blockIdx.x * 256 + threadIdx.x; i < d; i += gridDim.x * 256) y[size_t(r) * d + i] = 0;
 }
 
-int check_geom(const pmoe_geom* g) {
+int check_geom(const pmoe_geom* g, const void* slab) {
   PMOE_REQUIRE(g != nullptr, "null geometry");
   PMOE_REQUIRE(g->bits == 4 || g->bits == 6, "geometry: bits must be 4 or 6");
+  if (is_mx(g)) {
+    PMOE_REQUIRE(g->bits == 4, "geometry: group 32 (microscaled) has 4 bits");
+    PMOE_REQUIRE(g->hidden > 0 && g->hidden % 32 == 0 && g->inter > 0 && g->inter % 32 == 0,
+                 "geometry: hidden and inter must be multiples of 32");
+    PMOE_REQUIRE(g->hidden <= 8192 && g->inter <= 8192, "geometry: dims above 8192");
+    PMOE_REQUIRE((g->expert_bytes | g->off[PMOE_GATE_W] | g->off[PMOE_UP_W] |
+                  g->off[PMOE_DOWN_W]) % 16 == 0 && reinterpret_cast<uintptr_t>(slab) % 16 == 0,
+                 "geometry: microscaled weights must lie on 16 bytes");
+    return PMOE_OK;
+  }
   PMOE_REQUIRE(g->group == 64, "geometry: group must be 64");
   PMOE_REQUIRE(g->hidden > 0 && g->hidden % 64 == 0 && g->inter > 0 && g->inter % 64 == 0,
                "geometry: hidden and inter must be multiples of 64");
@@ -250,7 +280,7 @@ int check_route_cfg(const pmoe_route_cfg* rc) {
 // the two can be compared); a pinned prefill tile height keeps the GEMMs.
 bool stream_wanted(const pmoe_geom* g, const uint8_t* slab, int n, int kk, int n_experts,
                    int n_ids) {
-  if (!stream_covers(g, slab)) return false;
+  if (is_mx(g) || !stream_covers(g, slab)) return false;
   const char* v = getenv("PMOE_STREAM");
   if (v && (v[0] == '0' || v[0] == '1')) return v[0] == '1';
   const int64_t rows = int64_t(n) * kk, mib = 1 << 20;
@@ -273,6 +303,20 @@ int run_experts(const pmoe_geom* g, const uint8_t* slab, const int32_t* table, i
                 int max_rows_per_expert, const MoeWs& w, void* y, int y_f32, hipStream_t st) {
   const int rows = n * kk;
   const int n_ids = n_experts + (kk > k ? 1 : 0);
+  if (is_mx(g)) {
+    const int tm = mx_tile_rows(n, kk, n_experts);
+    if (int rc = dispatch_ext(inds, rows, k, kk, n_ids, w.order, w.counts, w.offsets, w.inv,
+                              w.active, w.n_active, tm, w.tiles, w.n_tiles, table, shared_slot,
+                              w.dws, w.dws_bytes, st))
+      return rc;
+    MxPlan p{};
+    p.geom = g, p.slab = slab, p.x = x, p.n = n, p.kk = kk;
+    p.order = w.order, p.tiles = w.tiles, p.n_tiles = w.n_tiles;
+    p.max_tiles = rows / tm + std::min(rows, n_ids) + 1;
+    p.xpair = w.xpair, p.xthird = w.xthird, p.xscale = w.xscale, p.xsteps = w.xsteps;
+    p.hpair = w.hpair, p.hscale = w.hscale, p.y = static_cast<uint16_t*>(y);
+    return mx_experts(p, st);
+  }
   const bool stream = stream_wanted(g, slab, n, kk, n_experts, n_ids);
   const bool prefill = !stream && prefill_wanted(g, n, kk, n_ids);
   const int tm = stream ? stream_tile_rows() : prefill ? prefill_tile_rows(n, kk, n_experts) : 0;
@@ -465,7 +509,7 @@ int experts_and_combine(const pmoe_geom* g, const uint8_t* slab, const int32_t* 
                         uint16_t* out, const MoeWs& w, hipStream_t st) {
   const int shared = shared_slot >= 0 ? 1 : 0;
   const int kk = k + shared;
-  if (n == 1 && k == kXcdCount && !(shared && shared_gate)) {
+  if (n == 1 && k == kXcdCount && !is_mx(g) && !(shared && shared_gate)) {
     // one token, eight columns: the expert-per-XCD launch (same outputs)
     GemvArgs gu{};
     gu.slab = slab;
@@ -562,7 +606,7 @@ extern "C" int pmoe_switch_glu(const pmoe_geom* g, const void* slab, const int32
                                int n_experts, const void* x, const int32_t* inds, int n, int k,
                                void* y, void* ws, size_t ws_bytes, void* stream) {
   pmoe::clear_error();
-  int rc = pmoe::check_geom(g);
+  int rc = pmoe::check_geom(g, slab);
   if (rc) return rc;
   PMOE_REQUIRE(slab && table && x && inds && y, "switch_glu: null pointer");
   PMOE_REQUIRE(n >= 0 && k > 0 && n_experts > 0 && n_experts <= 1023, "switch_glu: bad shape");
@@ -588,7 +632,7 @@ extern "C" int pmoe_moe_experts(const pmoe_geom* g, const void* slab, const int3
                                 const void* shared_gate, void* out, void* ws, size_t ws_bytes,
                                 void* stream) {
   pmoe::clear_error();
-  int rc = pmoe::check_geom(g);
+  int rc = pmoe::check_geom(g, slab);
   if (rc) return rc;
   PMOE_REQUIRE(slab && table && x && inds && weights && out, "moe_experts: null pointer");
   PMOE_REQUIRE(n >= 0 && k > 0 && n_experts > 0 && n_experts <= 1023, "moe_experts: bad shape");
@@ -610,7 +654,7 @@ extern "C" int pmoe_moe_block(const pmoe_geom* g, const pmoe_route_cfg* rc_cfg, 
                               const void* shared_gate, void* out, int32_t* inds_out,
                               float* weights_out, void* ws, size_t ws_bytes, void* stream) {
   pmoe::clear_error();
-  int rc = pmoe::check_geom(g);
+  int rc = pmoe::check_geom(g, slab);
   if (rc) return rc;
   PMOE_REQUIRE(rc_cfg != nullptr, "moe_block: null routing config");
   PMOE_REQUIRE(slab && table && gate_w && x && out && inds_out && weights_out,
@@ -629,7 +673,8 @@ extern "C" int pmoe_moe_block(const pmoe_geom* g, const pmoe_route_cfg* rc_cfg, 
   const uint16_t* xb = static_cast<const uint16_t*>(x);
   const int kk = k + shared;
   const bool decode = n * kk <= pmoe::kRouteMaxRows && e + 1 <= pmoe::kRouteMaxIds &&
-                      k <= pmoe::kRouteMaxK && !pmoe::prefill_wanted(g, n, kk, e + shared) &&
+                      k <= pmoe::kRouteMaxK && !pmoe::is_mx(g) &&
+                      !pmoe::prefill_wanted(g, n, kk, e + shared) &&
                       (rc_cfg->scoring == PMOE_SCORE_SOFTMAX ||
                        (e <= pmoe::kRouteMaxSigE && rc_cfg->topk_group <= 8));
   if (decode) {
@@ -718,7 +763,7 @@ extern "C" int pmoe_moe_block_noalloc(const pmoe_geom* g, const pmoe_route_cfg* 
                                       const void* shared_gate, void* out, int32_t* inds_out,
                                       float* weights_out, void* stream) {
   pmoe::clear_error();
-  int rc = pmoe::check_geom(g);
+  int rc = pmoe::check_geom(g, slab);
   if (rc) return rc;
   PMOE_REQUIRE(rc_cfg != nullptr, "moe_block_noalloc: null routing config");
   PMOE_REQUIRE(n >= 0 && rc_cfg->top_k > 0 && rc_cfg->n_experts > 0 &&

@@ -1,0 +1,52 @@
+// Launch interface of the microscaled 4-bit experts (mx_experts.hip).
+#pragma once
+
+#include "pmoe_internal.h"
+
+namespace pmoe {
+
+// Whether a geometry's experts are microscaled 4-bit (include/pmoe.h).
+inline bool is_mx(const pmoe_geom* g) { return g->group == 32; }
+
+// One grouped product over an expert's rows: features [features, cols] of the
+// slot times activation pieces.
+struct MxArgs {
+  const uint8_t* slab;
+  int64_t expert_bytes;
+  int64_t w0, s0, w1, s1;  // component offsets; 1: the up projection
+  const int4* tiles;       // {slot, first row, rows, offset}
+  const int32_t* n_tiles;
+  const int32_t* order;    // sorted position -> flat row
+  int kk, features, cols;
+  const uint8_t* pair;     // [rows, cols / 32, 48]
+  const uint8_t* third;    // [rows, cols / 32, 32]
+  const uint8_t* ascale;   // [rows, cols / 32]
+  uint8_t* hpair;          // gate/up out: [sorted row, features / 32, 48]
+  uint8_t* hscale;
+  uint16_t* y;             // down out: bf16 [flat row, features]
+};
+
+struct MxPlan {
+  const pmoe_geom* geom;
+  const uint8_t* slab;
+  const uint16_t* x;  // bf16 [n, hidden]
+  int n, kk;
+  const int32_t* order;
+  const int4* tiles;
+  const int32_t* n_tiles;
+  int max_tiles;
+  // scratch: the tokens' pieces, the sorted rows' intermediate
+  uint8_t *xpair, *xthird, *xscale;
+  uint16_t* xsteps;  // [n, 4]
+  uint8_t *hpair, *hscale;
+  uint16_t* y;  // bf16 [n * kk, hidden]
+};
+
+// Rows of the dispatch's tiles for such a call, and the fewest that any has.
+int mx_tile_rows(int n, int kk, int n_experts);
+int mx_min_tile_rows();
+// Split, gate/up, down over the dispatch's tiles; rows whose expert is not
+// resident come out zero.
+int mx_experts(const MxPlan& p, hipStream_t st);
+
+}  // namespace pmoe

@@ -1,0 +1,117 @@
+// Activations as sums of 6-bit floats under shared powers of two, the form in
+// which the scaled matrix instructions take them beside 4-bit weights.
+//
+// A group of 32 activations gets a power of two 2^e that brings its largest
+// magnitude into [4, 8), and each value a is written as
+//
+//   a = 2^e (p0 + p1 / 16 + p2 / 256) + rest
+//
+// with pieces of 1 sign, 2 exponent and 3 mantissa bits (E2M3: steps of 1/8 up
+// to 2, 1/4 up to 4, 1/2 up to 7.5), each the nearest to what the ones before
+// leave over.  Two pieces hold a bf16 value of at least an eighth of the
+// group's largest exactly and any other to 2^-8 2^e, i.e. to 2^-10 of the
+// largest; an fp32 value is off by at most 2^-9 of itself where it is among the
+// largest and by 2^-10 of the largest elsewhere, as a rounding to bf16 would be
+// (2^-9).  The third piece is kept only where one value stands out of its group
+// (its square is more than the sum of the other 31, in trained models the few
+// channels with huge activations), so that the other 31 are not rounded
+// to a step that it sets: they are then off by at most 2^-14 of the largest.
+//
+// A group that holds an infinity or a NaN gets the scale 255 (not a number).
+#pragma once
+
+#include "pmoe_internal.h"
+
+namespace pmoe {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x32 __attribute__((ext_vector_type(32)));
+typedef uint32_t u32x6 __attribute__((ext_vector_type(6)));
+
+constexpr int kMxGroup = 32;
+constexpr int kMxPieceBytes = 24;     // 32 values of 6 bits
+constexpr int kMxPairBytes = 48;      // p0, p1 of a group
+constexpr int kMxThirdBytes = 32;     // p2 of a group, padded to whole 16 bytes
+// The least scale byte of p0: the last piece's, 4 or 8 below, is at least 1.
+constexpr int kMxMinScalePair = 5, kMxMinScaleThird = 9;
+
+// 32 floats over 2^x to E2M3, nearest even.  The instruction takes the even
+// and the odd values apart, and writes its result while it still reads its
+// operands, which the compiler does not know: the empty statement keeps the
+// operands alive so that the result gets registers of its own.
+__device__ __forceinline__ u32x6 mx_to_fp6(const float (&v)[32], float scale) {
+  f32x16 even, odd;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) even[i] = v[2 * i], odd[i] = v[2 * i + 1];
+  u32x6 r = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, scale);
+  asm volatile("" : "+v"(r) : "v"(even), "v"(odd), "v"(scale));
+  return r;
+}
+
+__device__ __forceinline__ f32x32 mx_from_fp6(u32x6 q, float scale) {
+  f32x32 r = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(q, scale);
+  asm volatile("" : "+v"(r) : "v"(q), "v"(scale));  // as above
+  return r;
+}
+
+__device__ __forceinline__ float mx_pow2(int biased) {
+  return __uint_as_float(uint32_t(biased) << 23);
+}
+
+// The scale byte of a group and its first two pieces; v is left with the rest.
+// With THIRD also p2 (zeros where no value stands out, and then false).
+template <bool THIRD>
+__device__ __forceinline__ bool mx_split(float (&v)[32], int& scale, u32x6& p0, u32x6& p1,
+                                         u32x6& p2) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+  const int e = int(top >> 23);
+  const int s = max(e - 2, THIRD ? kMxMinScaleThird : kMxMinScalePair);
+  bool peak = false;
+  if constexpr (THIRD) {
+    // in units of 2^s the squares neither overflow nor vanish
+    const float inv = mx_pow2(254 - s);
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const float t = v[i] * inv;
+      sum = __builtin_fmaf(t, t, sum);
+    }
+    const float t = __uint_as_float(top) * inv;
+    peak = 2.0f * t * t > sum;
+  }
+  const float f = mx_pow2(s);
+  p0 = mx_to_fp6(v, f);
+  f32x32 b = mx_from_fp6(p0, f);
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] -= b[i];
+  const float f1 = mx_pow2(s - 4);
+  p1 = mx_to_fp6(v, f1);
+  p2 = u32x6{0, 0, 0, 0, 0, 0};
+  if constexpr (THIRD) {
+    if (peak) {
+      b = mx_from_fp6(p1, f1);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] -= b[i];
+      p2 = mx_to_fp6(v, mx_pow2(s - 8));
+    }
+  }
+  scale = e == 255 ? 255 : s;
+  return peak;
+}
+
+__device__ __forceinline__ void mx_store_pair(uint8_t* dst, u32x6 p0, u32x6 p1) {
+  uint4* d = reinterpret_cast<uint4*>(dst);
+  d[0] = make_uint4(p0[0], p0[1], p0[2], p0[3]);
+  d[1] = make_uint4(p0[4], p0[5], p1[0], p1[1]);
+  d[2] = make_uint4(p1[2], p1[3], p1[4], p1[5]);
+}
+
+__device__ __forceinline__ void mx_store_third(uint8_t* dst, u32x6 p2) {
+  uint4* d = reinterpret_cast<uint4*>(dst);
+  d[0] = make_uint4(p2[0], p2[1], p2[2], p2[3]);
+  d[1] = make_uint4(p2[4], p2[5], 0, 0);
+}
+
+}  // namespace pmoe

@@ -18,6 +18,10 @@ enum KernelId {
   K_DECODE_FUSED,
   K_DECODE_XCD,
   K_EXPERTS_XCD,
+  K_MX_SPLIT,
+  K_MX_GATEUP,
+  K_MX_DOWN,
+  K_BLOCK_NORM,
   K_COUNT
 };
 

@@ -1459,7 +1459,7 @@ int prefill_experts(const pmoe_geom* g, const uint8_t* slab, const uint16_t* x, 
 
 extern "C" int pmoe_prefill_wide(const pmoe_geom* g, const void* slab, const void* x, int n,
                                  int kk, int n_experts) {
-  if (!g || n <= 0 || kk <= 0 || n_experts <= 0) return 0;
+  if (!g || g->group != 64 || n <= 0 || kk <= 0 || n_experts <= 0) return 0;
   return pmoe::prefill_tile_rows(n, kk, n_experts) == pmoe::kTileM &&
                  pmoe::prefill_wide(g, slab, x, n, kk, n_experts)
              ? 1

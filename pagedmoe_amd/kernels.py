@@ -38,6 +38,20 @@ def _stream():
     return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
 
 
+def _stream_of(t):
+    """The current stream for work on t, which must be on the current device
+    (launches go there)."""
+    if t.device.index != torch._C._cuda_getDevice():
+        raise ValueError(f"tensors on {t.device}, but the current device is "
+                         f"cuda:{torch._C._cuda_getDevice()}: call under torch.cuda.device")
+    return _stream()
+
+
+def _same_device(a, b, name):
+    if a.device != b.device:
+        raise ValueError(f"{name}: on {b.device}, the other tensors on {a.device}")
+
+
 def _need(t, dtype, name, ndim=None):
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a tensor")
@@ -181,6 +195,55 @@ def dequant(q, scales, biases, bits: int, group: int = 64) -> torch.Tensor:
     return out
 
 
+_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+def mx4_quantize(w: torch.Tensor, out=None):
+    """w [R, C] of fp32, bf16 or fp16 -> (q int32 [R, C/8], scales uint8
+    [R, C/32]) in the microscaled 4-bit format (pmoe_mx4_quantize).  ``out`` =
+    (q, scales) contiguous tensors to write into (e.g. slab views)."""
+    if not isinstance(w, torch.Tensor) or w.dtype not in _DTYPES:
+        raise TypeError("w: expected an fp32, bf16 or fp16 tensor")
+    _need(w, w.dtype, "w", 2)
+    r, c = w.shape
+    if c == 0 or c % 32:
+        raise ValueError("columns must be a multiple of the group size, 32")
+    if out is None:
+        q = torch.empty((r, c // 8), dtype=torch.int32, device=w.device)
+        s = torch.empty((r, c // 32), dtype=torch.uint8, device=w.device)
+    else:
+        q, s = out
+        for t, dt, shape, name in ((q, torch.int32, (r, c // 8), "q"),
+                                   (s, torch.uint8, (r, c // 32), "scales")):
+            _need(t, dt, name)
+            if tuple(t.shape) != shape:
+                raise ValueError(f"{name}: expected {shape}, got {tuple(t.shape)}")
+            _same_device(w, t, name)
+    if r:
+        check(lib().pmoe_mx4_quantize(_ptr(w), _DTYPES[w.dtype], r, c, _ptr(q), _ptr(s),
+                                      _stream_of(w)), "pmoe_mx4_quantize")
+    return q, s
+
+
+def mx4_dequant(q: torch.Tensor, scales: torch.Tensor, dtype=torch.bfloat16) -> torch.Tensor:
+    """The values [R, C] of microscaled 4-bit words q [R, C/8] and scales
+    [R, C/32], rounded once to ``dtype`` (fp32, bf16 or fp16)."""
+    _need(q, torch.int32, "q", 2)
+    _need(scales, torch.uint8, "scales", 2)
+    if dtype not in _DTYPES:
+        raise TypeError("dtype: expected fp32, bf16 or fp16")
+    r, c = q.shape[0], q.shape[1] * 8
+    if c == 0 or c % 32 or tuple(scales.shape) != (r, c // 32):
+        raise ValueError(f"scales: expected {(r, c // 32)} for words {tuple(q.shape)} of whole "
+                         f"groups, got {tuple(scales.shape)}")
+    _same_device(q, scales, "scales")
+    out = torch.empty((r, c), dtype=dtype, device=q.device)
+    if r:
+        check(lib().pmoe_mx4_dequant(_ptr(q), _ptr(scales), r, c, _DTYPES[dtype], _ptr(out),
+                                     _stream_of(q)), "pmoe_mx4_dequant")
+    return out
+
+
 # ---------------------------------------------------------------- experts
 
 def moe_workspace(g: Geom, n: int, k: int, shared: int, n_experts: int, device,
@@ -290,6 +353,8 @@ def switch_glu(g: Geom, slab: torch.Tensor, table, n_experts: int, x: torch.Tens
     if x.shape != (n, g.hidden):
         raise ValueError(f"x must be [{n}, {g.hidden}], got {tuple(x.shape)}")
     y = torch.empty((n, k, g.hidden), dtype=torch.bfloat16, device=x.device)
+    if n == 0:
+        return y
     ws = moe_workspace(g, n, k, 0, n_experts, x.device)
     check(lib().pmoe_switch_glu(ctypes.byref(g), _ptr(slab), _table_ptr(table), n_experts,
                                 _ptr(x), _ptr(inds), n, k, _ptr(y), _ptr(ws), ws.numel(),
@@ -314,6 +379,8 @@ def moe_experts(g: Geom, slab, table, n_experts: int, x, inds, weights, shared_s
     _need(weights, torch.float32, "weights", 2)
     n, k = inds.shape
     out = torch.empty((n, g.hidden), dtype=torch.bfloat16, device=x.device)
+    if n == 0:
+        return out
     ws = moe_workspace(g, n, k, int(shared_slot >= 0), n_experts, x.device)
     check(lib().pmoe_moe_experts(ctypes.byref(g), _ptr(slab), _table_ptr(table), n_experts,
                                  _ptr(x), _ptr(inds), _ptr(weights), n, k, int(shared_slot),

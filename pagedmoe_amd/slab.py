@@ -4,7 +4,8 @@ Counterpart of the reference's ``SlabStore`` (slab.py:82-183).  The reference
 keeps one ``[slots, *expert_shape]`` array per component in unified memory
 and preads into it.  Here a slab is ONE device allocation of
 ``slots * expert_bytes`` bytes laid out expert-major: slot s holds the nine
-components of one expert back to back (``pmoe_geom.off``), so a miss is a
+components of one expert back to back (``pmoe_geom.off``; six in the microscaled 4-bit format, group 32,
+which has no biases), so a miss is a
 single contiguous host->HBM copy and every kernel addresses an expert as
 ``base + slot * expert_bytes``.  ``compute(name)`` still hands out the
 reference's ``[slots, *shape]`` view of one component (a strided view, no
@@ -15,27 +16,30 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import COMPONENTS, Geom, geom as make_geom
+from ._lib import COMPONENTS, Geom, geom as make_geom, is_mx
 
 
 def component_specs(g: Geom) -> dict:
     """name -> (per-expert shape, torch dtype, nbytes, offset)."""
     d, i, b = g.hidden, g.inter, g.bits
     gs = g.group
+    st = torch.uint8 if is_mx(g) else torch.bfloat16
     shapes = {
         "gate_proj.weight": ((i, d * b // 32), torch.int32),
-        "gate_proj.scales": ((i, d // gs), torch.bfloat16),
+        "gate_proj.scales": ((i, d // gs), st),
         "gate_proj.biases": ((i, d // gs), torch.bfloat16),
         "up_proj.weight": ((i, d * b // 32), torch.int32),
-        "up_proj.scales": ((i, d // gs), torch.bfloat16),
+        "up_proj.scales": ((i, d // gs), st),
         "up_proj.biases": ((i, d // gs), torch.bfloat16),
         "down_proj.weight": ((d, i * b // 32), torch.int32),
-        "down_proj.scales": ((d, i // gs), torch.bfloat16),
+        "down_proj.scales": ((d, i // gs), st),
         "down_proj.biases": ((d, i // gs), torch.bfloat16),
     }
     out = {}
     for c, name in enumerate(COMPONENTS):
         shape, dt = shapes[name]
+        if g.nbytes[c] == 0:  # the microscaled format's biases
+            continue
         out[name] = (shape, dt, int(g.nbytes[c]), int(g.off[c]))
     return out
 
@@ -50,14 +54,15 @@ class SlabStore:
         self.slots = int(slots)
         self.expert_bytes = int(g.expert_bytes)
         self.specs = component_specs(g)
-        self.names = tuple(COMPONENTS)
+        self.names = tuple(self.specs)
         alloc = torch.zeros if zero else torch.empty
         self.buf = alloc(self.slots * self.expert_bytes, dtype=torch.uint8, device=device)
         self.nbytes = self.buf.numel()
 
     @classmethod
-    def for_shape(cls, hidden: int, inter: int, bits: int, slots: int, device="cuda"):
-        return cls(make_geom(hidden, inter, bits), slots, device)
+    def for_shape(cls, hidden: int, inter: int, bits: int, slots: int, device="cuda",
+                  group: int = 64):
+        return cls(make_geom(hidden, inter, bits, group), slots, device)
 
     @property
     def data_ptr(self) -> int:
@@ -108,7 +113,7 @@ class SlabStore:
             if not isinstance(src, torch.Tensor):
                 import numpy as np
                 arr = np.ascontiguousarray(src)
-                arr = arr.view(np.int32 if dt == torch.int32 else np.int16)
+                arr = arr.view({torch.int32: np.int32, torch.uint8: np.uint8}.get(dt, np.int16))
                 src = torch.from_numpy(arr)
             src = src.reshape(shape)
             if src.dtype != dt:
@@ -119,6 +124,10 @@ class SlabStore:
         """Quantize fp32 weights w ([out, in] of projection `proj`) straight
         into slot's components (no staging copy)."""
         from . import kernels
+        if is_mx(self.geom):
+            kernels.mx4_quantize(w, out=(self.expert(proj + ".weight", slot),
+                                         self.expert(proj + ".scales", slot)))
+            return
         kernels.quantize(w, self.geom.bits, self.geom.group,
                          out=(self.expert(proj + ".weight", slot),
                               self.expert(proj + ".scales", slot),

@@ -32,7 +32,8 @@ PROJS = ("gate_proj", "up_proj", "down_proj")
 class QuantizedSwitchGLU(nn.Module):
     """Resident stacked experts: E affine-quantized SwiGLU experts (plus an
     optional shared expert in slot E) in one slab, expert e in slot e.  The
-    resident counterpart of mlx-lm's SwitchGLU over QuantizedSwitchLinear."""
+    resident counterpart of mlx-lm's SwitchGLU over QuantizedSwitchLinear.
+    ``group=32`` (with 4 bits) holds them in the microscaled 4-bit format."""
 
     def __init__(self, hidden: int, inter: int, n_experts: int, bits: int = 4, group: int = 64,
                  n_shared: int = 0, device="cuda"):
@@ -516,19 +517,20 @@ def build_cache_for(model: nn.Module, slots: int, model_path=None, **kw) -> Expe
     n_shared = first.n_shared
     g = first.geom
     for _, m in glus:
-        if (m.hidden, m.inter, m.bits, m.n_experts, m.n_shared) != (
-                first.hidden, first.inter, first.bits, first.n_experts, n_shared):
+        if (m.hidden, m.inter, m.bits, m.geom.group, m.n_experts, m.n_shared) != (
+                first.hidden, first.inter, first.bits, g.group, first.n_experts, n_shared):
             raise ValueError("all MoE layers must share one expert shape")
     if model_path is not None:
         store = HostExpertStore.from_checkpoint(model_path)
         sg = store.geom
-        if (store.n_layers, store.n_experts, sg.hidden, sg.inter, sg.bits) != (
-                len(glus), first.n_experts, first.hidden, first.inter, first.bits):
+        if (store.n_layers, store.n_experts, sg.hidden, sg.inter, sg.bits, sg.group) != (
+                len(glus), first.n_experts, first.hidden, first.inter, first.bits, g.group):
             store.close()
             raise ValueError(f"{model_path}: {store.n_layers} MoE layers of {store.n_experts} "
-                             f"experts ({sg.hidden}/{sg.inter}/{sg.bits}-bit) do not match the "
-                             f"model's {len(glus)} layers of {first.n_experts} "
-                             f"({first.hidden}/{first.inter}/{first.bits}-bit)")
+                             f"experts ({sg.hidden}/{sg.inter}/{sg.bits}-bit in groups of "
+                             f"{sg.group}) do not match the model's {len(glus)} layers of "
+                             f"{first.n_experts} ({first.hidden}/{first.inter}/{first.bits}-bit "
+                             f"in groups of {g.group})")
     else:
         store = HostExpertStore(g, len(glus), first.n_experts)
         for li, (_, m) in enumerate(glus):
