@@ -307,6 +307,46 @@ int pmoe_combine(const void* y, const float* weights, int n, int k, int hidden,
                  const void* shared_y, const float* shared_logit, void* out,
                  void* stream);
 
+/* ---- norms around a block (mlx-lm's decoder layers run them as nn.RMSNorm
+ *      before the block, the residual add after it and the next layer's norm;
+ *      the reference leaves them to mlx) ------------------------------------ */
+
+/* What a gate of pmoe_block_join multiplies: nothing, each channel ([hidden]),
+ * each token ([n]) or each element ([n, hidden]). */
+enum { PMOE_GATE_NONE = 0, PMOE_GATE_CHANNEL, PMOE_GATE_TOKEN, PMOE_GATE_ELEMENT };
+
+typedef struct {
+  int32_t stream_dtype;  /* residual and out: PMOE_F32 or PMOE_BF16 */
+  int32_t weight_dtype;  /* both norms' weights */
+  int32_t gate_kind;     /* PMOE_GATE_* */
+  int32_t gate_dtype;
+  int32_t gate_sigmoid;  /* gate by sigmoid(gate) */
+  int32_t unit_offset;   /* norm weights are 1 + w (zero-centred) */
+  float residual_scale, branch_scale;
+  float eps;             /* of both norms */
+} pmoe_join;
+
+/* h = w * x / sqrt(mean(x^2) + eps) over each row of x [n, hidden] (fp32 or
+ * bf16; weight [hidden] fp32 or bf16; 1 + weight with unit_offset), bf16 out.
+ * hidden: 1..16384.  The sum of a row's squares must stay inside fp32. */
+int pmoe_block_norm(const void* x, int x_dtype, const void* weight, int weight_dtype, int n,
+                    int hidden, float eps, int unit_offset, void* h, void* stream);
+
+/* After a block, in one pass: out = residual_scale * residual + branch_scale *
+ * gate * norm(y) and h = norm(out), where
+ *   y      bf16 [n, k, hidden] combined with weights fp32 [n, k] in slot order
+ *          as pmoe_combine does (NULL: k = 1 and y as it is), plus shared_y
+ *          bf16 [n, hidden] (NULL: none) times 1 or sigmoid(shared_logit[n])
+ *   norm   the RMS norm with post_weight (NULL: none) and with next_weight
+ *          (NULL: no h; h bf16 [n, hidden])
+ *   gate   of gate_kind (NULL: none)
+ * residual and out are [n, hidden] of stream_dtype; out may be residual.  All in
+ * fp32, each result rounded once (h from out before its rounding). */
+int pmoe_block_join(const pmoe_join* j, const void* residual, const void* y, const float* weights,
+                    const void* shared_y, const float* shared_logit, const void* post_weight,
+                    const void* gate, const void* next_weight, int n, int k, int hidden, void* out,
+                    void* h, void* stream);
+
 /* Closed-stitch miss count (replaces the per-layer miss sum of
  * _closed_forward, streaming.py:905-935, and the token wrapper's one read of
  * it, _closed_call :2843-2870): *counter += the number of ids[0..n) with

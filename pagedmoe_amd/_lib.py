@@ -23,6 +23,7 @@ COMPONENTS = (
 SCORE_SOFTMAX = 0
 SCORE_SIGMOID = 1
 F32, BF16, F16 = 0, 1, 2
+GATE_NONE, GATE_CHANNEL, GATE_TOKEN, GATE_ELEMENT = 0, 1, 2, 3
 
 
 class PmoeError(RuntimeError):
@@ -51,6 +52,12 @@ class RouteCfg(ctypes.Structure):
         ("topk_group", ctypes.c_int32),
         ("routed_scale", ctypes.c_float),
     ]
+
+
+class Join(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in (
+        "stream_dtype", "weight_dtype", "gate_kind", "gate_dtype", "gate_sigmoid",
+        "unit_offset")] + [(n, ctypes.c_float) for n in ("residual_scale", "branch_scale", "eps")]
 
 
 class SlabStats(ctypes.Structure):
@@ -103,6 +110,9 @@ SIGNATURES = {
     "pmoe_moe_block_noalloc": (_I, [ctypes.POINTER(Geom), ctypes.POINTER(RouteCfg), _P, _P, _P,
                                     _P, _P, _P, _I, _I, _P, _P, _P, _P, _P]),
     "pmoe_combine": (_I, [_P, _P, _I, _I, _I, _P, _P, _P, _P]),
+    "pmoe_block_norm": (_I, [_P, _I, _P, _I, _I, _I, _F, _I, _P, _P]),
+    "pmoe_block_join": (_I, [ctypes.POINTER(Join), _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I,
+                             _P, _P, _P]),
     "pmoe_count_missing": (_I, [_P, _P, _I, _I, _P, _P]),
     "pmoe_slab_create": (_I, [ctypes.POINTER(_P), _I, _I, _I, _F, _I, _I]),
     "pmoe_slab_destroy": (_I, [_P]),

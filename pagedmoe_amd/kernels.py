@@ -411,6 +411,113 @@ def combine(y: torch.Tensor, weights: torch.Tensor, shared_y=None, shared_logit=
     return out
 
 
+def _stream_dtype(t, name, dtype=None):
+    """The ABI's type of an fp32 or bf16 tensor (of ``dtype``, if given)."""
+    if not isinstance(t, torch.Tensor) or t.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"{name}: expected an fp32 or bf16 tensor")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+    return _DTYPES[t.dtype]
+
+
+def _like(t, ref, shape, name, dtype=None):
+    """t is contiguous, of ``shape`` (and ``dtype``), on ref's device."""
+    _need(t, t.dtype if dtype is None else dtype, name)
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name}: expected {tuple(shape)}, got {tuple(t.shape)}")
+    _same_device(ref, t, name)
+
+
+def block_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
+               unit_offset: bool = False) -> torch.Tensor:
+    """h [N, D] bf16: the RMS norm of a residual stream x [N, D] (fp32 or
+    bf16) with weight [D] (fp32 or bf16; 1 + weight with unit_offset), the
+    input of a block (pmoe_block_norm)."""
+    xd, wd = _stream_dtype(x, "x"), _stream_dtype(weight, "weight")
+    _need(x, x.dtype, "x", 2)
+    n, d = x.shape
+    _like(weight, x, (d,), "weight")
+    h = torch.empty((n, d), dtype=torch.bfloat16, device=x.device)
+    if n:
+        check(lib().pmoe_block_norm(_ptr(x), xd, _ptr(weight), wd, n, d, float(eps),
+                                    int(bool(unit_offset)), _ptr(h), _stream_of(x)),
+              "pmoe_block_norm")
+    return h
+
+
+def block_join(residual: torch.Tensor, y: torch.Tensor, weights=None, *, shared_y=None,
+               shared_logit=None, post_weight=None, gate=None, gate_sigmoid: bool = False,
+               residual_scale: float = 1.0, branch_scale: float = 1.0, next_weight=None,
+               eps: float = 1e-6, unit_offset: bool = False, out=None):
+    """(out, h): what follows a block, in one pass (pmoe_block_join).
+
+    out [N, D] (residual's type, fp32 or bf16) = residual_scale * residual +
+    branch_scale * gate * norm(y); h [N, D] bf16 = norm(out), or None without
+    ``next_weight``.  ``y``: a block's outputs bf16 [N, D], or its per-slot
+    outputs [N, K, D] with routing ``weights`` fp32 [N, K] (and ``shared_y``,
+    ``shared_logit``), combined as ``combine`` does.  ``post_weight`` /
+    ``next_weight`` [D] (one type, fp32 or bf16) are the RMS norms'; without
+    ``post_weight`` y is not normed.  ``gate`` (fp32 or bf16): [D] per channel,
+    [N, 1] per token or [N, D], by itself or its sigmoid.  ``out`` may be
+    ``residual`` itself; it overlaps no other input."""
+    j = _lib.Join()
+    j.stream_dtype = _stream_dtype(residual, "residual")
+    _need(residual, residual.dtype, "residual", 2)
+    n, d = residual.shape
+    _need(y, torch.bfloat16, "y")
+    _same_device(residual, y, "y")
+    if weights is None:
+        k = 1
+        _like(y, residual, (n, d), "y")
+    else:
+        if y.dim() != 3:
+            raise ValueError(f"y: expected [N, K, D] with weights, got {tuple(y.shape)}")
+        k = y.shape[1]
+        _like(y, residual, (n, k, d), "y")
+        _like(weights, residual, (n, k), "weights", torch.float32)
+    if shared_y is not None:
+        _like(shared_y, residual, (n, d), "shared_y", torch.bfloat16)
+    if shared_logit is not None:
+        _need(shared_logit, torch.float32, "shared_logit")
+        _same_device(residual, shared_logit, "shared_logit")
+        if shared_y is None or shared_logit.numel() != n:
+            raise ValueError("shared_logit must hold N values, beside shared_y")
+    norms = [(t, name) for t, name in ((post_weight, "post_weight"), (next_weight, "next_weight"))
+             if t is not None]
+    for t, name in norms:
+        j.weight_dtype = _stream_dtype(t, name, norms[0][0].dtype)
+        _like(t, residual, (d,), name)
+    if gate is not None:
+        j.gate_dtype = _stream_dtype(gate, "gate")
+        shape = tuple(gate.shape)
+        if shape == (d,):
+            j.gate_kind = _lib.GATE_CHANNEL
+        elif shape == (n, 1):
+            j.gate_kind = _lib.GATE_TOKEN
+        elif shape == (n, d):
+            j.gate_kind = _lib.GATE_ELEMENT
+        else:
+            raise ValueError(f"gate: expected {(d,)}, {(n, 1)} or {(n, d)}, got {shape}")
+        _like(gate, residual, shape, "gate")
+    j.gate_sigmoid = int(bool(gate_sigmoid))
+    j.unit_offset = int(bool(unit_offset))
+    j.residual_scale, j.branch_scale = float(residual_scale), float(branch_scale)
+    j.eps = float(eps)
+    if out is None:
+        out = torch.empty_like(residual)
+    else:
+        _like(out, residual, (n, d), "out", residual.dtype)
+    h = None
+    if next_weight is not None:
+        h = torch.empty((n, d), dtype=torch.bfloat16, device=residual.device)
+    if n:
+        check(lib().pmoe_block_join(
+            ctypes.byref(j), _ptr(residual), _ptr(y), _ptr(weights), _ptr(shared_y),
+            _ptr(shared_logit), _ptr(post_weight), _ptr(gate), _ptr(next_weight), n, k, d,
+            _ptr(out), _ptr(h), _stream_of(residual)), "pmoe_block_join")
+    return out, h
+
+
 def route_cfg(scoring: str, n_experts: int, top_k: int, norm_topk_prob: bool = True,
               n_group: int = 1, topk_group: int = 1, routed_scale: float = 1.0) -> RouteCfg:
     rc = RouteCfg()

@@ -318,8 +318,15 @@ class _MoEBlock(nn.Module):
         return None
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        shape = x.shape
-        x2 = x.reshape(-1, shape[-1]).to(torch.bfloat16).contiguous()
+        x2 = x.reshape(-1, x.shape[-1]).to(torch.bfloat16).contiguous()
+        y, w, shared_y, shared_logit = self.mixture(x2)
+        out = y if w is None else K.combine(y, w, shared_y, shared_logit)
+        return out.reshape(x.shape)
+
+    def mixture(self, x2: torch.Tensor):
+        """The block on rows x2 [N, D] bf16: (out [N, D], None, None, None), or
+        where the experts ran in several passes their per-slot outputs and what
+        combines them (y [N, K, D], weights [N, K], shared_y, shared_logit)."""
         g, slab, table, n_exp, shared_slot = _experts_of(self.switch_mlp)
         if not self.use_shared:
             shared_slot = -1
@@ -342,7 +349,7 @@ class _MoEBlock(nn.Module):
             else:
                 sm.ring.count_missing(tab, inds)
             self.last_routing = (inds, w)
-            return out.reshape(shape)
+            return out, None, None, None
         if isinstance(sm, StreamedSwitchGLU) and not sm.cache.stitched:
             # route, then make the routed experts resident, then compute
             logits = K.router_logits(x2, self.gate_weight, self.logit_bias)
@@ -374,26 +381,25 @@ class _MoEBlock(nn.Module):
                                    torch.where(keep, inds, torch.full_like(inds, -1)))
                 sm.cache.note_compute(sm.layer_key)
                 y = y_g if y is None else torch.where(keep[..., None], y_g, y)
+            shared_y = shared_logit = None
             if out is None:
-                shared_y = shared_logit = None
                 if shared_slot >= 0:
                     one = torch.full((1,), shared_slot, dtype=torch.int32, device=x2.device)
                     zero = torch.zeros((x2.shape[0], 1), dtype=torch.int32, device=x2.device)
                     shared_y = K.switch_glu(g, slab, one, 1, x2, zero).reshape(x2.shape)
                     if sg is not None:
                         shared_logit = K.router_logits(x2, sg.reshape(1, -1)).reshape(-1)
-                out = K.combine(y, w, shared_y, shared_logit)
             if sm.ring is not None and x2.shape[0] <= config.DECODE_MAX_TOKENS:
                 sm.ring.speculate(sm.ring_index, x2)
             self.last_routing = (inds, w)
-            return out.reshape(shape)
+            return (y, w, shared_y, shared_logit) if out is None else (out, None, None, None)
         if table is None:
             table = sm.cache.table_ptr(sm.layer_key)
         out, inds, w = K.moe_block(g, rc, slab, table, self.gate_weight, x2,
                                    score_bias=self._score_bias(), logit_bias=self.logit_bias,
                                    shared_slot=shared_slot, shared_gate=sg)
         self.last_routing = (inds, w)
-        return out.reshape(shape)
+        return out, None, None, None
 
 
 def _predict_ids_softmax(blk, x, slack):
@@ -474,6 +480,52 @@ class SigmoidGroupMoEBlock(_MoEBlock):
         m = min(self.top_k + max(0, slack), 16, (e // self.n_group) * self.topk_group)
         return K.route_sigmoid_group_topk(logits, self.e_score_correction_bias, self.n_group,
                                           self.topk_group, m, True, 1.0)[0]
+
+
+class MoELayer(nn.Module):
+    """The MoE half of a decoder layer around one of the blocks above:
+
+        out = residual_scale * x + branch_scale * gate * post(block(pre(x)))
+
+    ``pre`` and ``post`` are RMS norms (``post_weight`` None: no second norm;
+    ``unit_offset``: weights are 1 + w), ``gate`` is per channel [D], per
+    token [N, 1] or per element [N, D] (None: none), itself or its sigmoid.
+    The norm before the block is one launch (``kernels.block_norm``), all that
+    follows it another (``kernels.block_join``), which also takes the combine
+    of a block whose experts ran in several passes."""
+
+    def __init__(self, block: _MoEBlock, pre_weight: torch.Tensor,
+                 post_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+                 gate_sigmoid: bool = False, residual_scale: float = 1.0,
+                 branch_scale: float = 1.0, eps: float = 1e-6, unit_offset: bool = False):
+        super().__init__()
+        self.block = block
+        self.pre_weight = pre_weight.contiguous()
+        self.post_weight = None if post_weight is None else post_weight.contiguous()
+        self.gate = None if gate is None else gate.contiguous()
+        self.gate_sigmoid = gate_sigmoid
+        self.residual_scale, self.branch_scale = residual_scale, branch_scale
+        self.eps, self.unit_offset = eps, unit_offset
+
+    def forward(self, x: torch.Tensor, gate: torch.Tensor | None = None,
+                h: torch.Tensor | None = None, next_weight: torch.Tensor | None = None):
+        """x [..., D] (a bf16 or fp32 residual stream) -> out like x.  ``gate``
+        replaces the layer's for this call.  With ``next_weight`` [D] also the
+        next norm of out, in the same launch: (out, h [..., D] bf16); that ``h``
+        is what the next layer takes here in place of its own first norm."""
+        d = x.shape[-1]
+        x2 = x.reshape(-1, d).contiguous()
+        if h is None:
+            h = K.block_norm(x2, self.pre_weight, self.eps, self.unit_offset)
+        y, w, shared_y, shared_logit = self.block.mixture(h.reshape(-1, d))
+        gate = self.gate if gate is None else gate
+        out, nh = K.block_join(
+            x2, y, w, shared_y=shared_y, shared_logit=shared_logit, post_weight=self.post_weight,
+            gate=gate, gate_sigmoid=self.gate_sigmoid, residual_scale=self.residual_scale,
+            branch_scale=self.branch_scale, next_weight=next_weight, eps=self.eps,
+            unit_offset=self.unit_offset)
+        out = out.reshape(x.shape)
+        return out if next_weight is None else (out, nh.reshape(x.shape))
 
 
 # ---------------------------------------------------------------- model surgery
