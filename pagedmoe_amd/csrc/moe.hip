@@ -304,14 +304,14 @@ int run_experts(const pmoe_geom* g, const uint8_t* slab, const int32_t* table, i
   const int rows = n * kk;
   const int n_ids = n_experts + (kk > k ? 1 : 0);
   if (is_mx(g)) {
-    const int tm = mx_tile_rows(n, kk, n_experts);
+    const int tm = mx_tile_rows(g, n, kk, n_experts);
     if (int rc = dispatch_ext(inds, rows, k, kk, n_ids, w.order, w.counts, w.offsets, w.inv,
                               w.active, w.n_active, tm, w.tiles, w.n_tiles, table, shared_slot,
                               w.dws, w.dws_bytes, st))
       return rc;
     MxPlan p{};
     p.geom = g, p.slab = slab, p.x = x, p.n = n, p.kk = kk;
-    p.order = w.order, p.tiles = w.tiles, p.n_tiles = w.n_tiles;
+    p.order = w.order, p.tile_rows = tm, p.tiles = w.tiles, p.n_tiles = w.n_tiles;
     p.max_tiles = rows / tm + std::min(rows, n_ids) + 1;
     p.xpair = w.xpair, p.xthird = w.xthird, p.xscale = w.xscale, p.xsteps = w.xsteps;
     p.hpair = w.hpair, p.hscale = w.hscale, p.y = static_cast<uint16_t*>(y);

@@ -21,6 +21,7 @@ struct MxArgs {
   const uint8_t* pair;     // [rows, cols / 32, 48]
   const uint8_t* third;    // [rows, cols / 32, 32]
   const uint8_t* ascale;   // [rows, cols / 32]
+  const uint16_t* asteps;  // [rows, 4]: bit s: step s of 128 has a third piece
   uint8_t* hpair;          // gate/up out: [sorted row, features / 32, 48]
   uint8_t* hscale;
   uint16_t* y;             // down out: bf16 [flat row, features]
@@ -32,6 +33,7 @@ struct MxPlan {
   const uint16_t* x;  // bf16 [n, hidden]
   int n, kk;
   const int32_t* order;
+  int tile_rows;  // of the tile list
   const int4* tiles;
   const int32_t* n_tiles;
   int max_tiles;
@@ -43,7 +45,7 @@ struct MxPlan {
 };
 
 // Rows of the dispatch's tiles for such a call, and the fewest that any has.
-int mx_tile_rows(int n, int kk, int n_experts);
+int mx_tile_rows(const pmoe_geom* g, int n, int kk, int n_experts);
 int mx_min_tile_rows();
 // Split, gate/up, down over the dispatch's tiles; rows whose expert is not
 // resident come out zero.

@@ -1,21 +1,30 @@
 // Activations as sums of 6-bit floats under shared powers of two, the form in
 // which the scaled matrix instructions take them beside 4-bit weights.
 //
-// A group of 32 activations gets a power of two 2^e that brings its largest
+// A group of 32 values gets a power of two 2^e that brings its largest
 // magnitude into [4, 8), and each value a is written as
 //
-//   a = 2^e (p0 + p1 / 16 + p2 / 256) + rest
+//   a = 2^e (p0 + p1 / 16 + p2 / 256) + rest     (tokens)
+//   a = 2^e (p0 + p1 / 32) + rest                (intermediates)
 //
 // with pieces of 1 sign, 2 exponent and 3 mantissa bits (E2M3: steps of 1/8 up
 // to 2, 1/4 up to 4, 1/2 up to 7.5), each the nearest to what the ones before
-// leave over.  Two pieces hold a bf16 value of at least an eighth of the
+// leave over.
+//
+// Tokens are bf16.  Two pieces hold a value of at least an eighth of the
 // group's largest exactly and any other to 2^-8 2^e, i.e. to 2^-10 of the
-// largest; an fp32 value is off by at most 2^-9 of itself where it is among the
-// largest and by 2^-10 of the largest elsewhere, as a rounding to bf16 would be
-// (2^-9).  The third piece is kept only where one value stands out of its group
-// (its square is more than the sum of the other 31, in trained models the few
-// channels with huge activations), so that the other 31 are not rounded
-// to a step that it sets: they are then off by at most 2^-14 of the largest.
+// largest.  The third is kept only where one value stands out of its group
+// (its square is more than the sum of the other 31's, in trained models the few
+// channels with huge activations), so that the others are not rounded to a
+// step that it sets: they are then off by at most 2^-14 of the largest.
+//
+// Intermediates are fp32.  The second piece's smaller unit makes its steps half
+// as wide where most values are (2^-9 2^e below 2, 2^-8 2^e below 4, 2^-7 2^e above,
+// and 2^-6 2^e where a value all but halves two steps of p0 and p1 ends at
+// 7.5): off by 2^-8 of the group's largest at most and by as much as a
+// rounding to bf16 would be on average.  A largest value of 7.75 2^e and more
+// takes the next power of two, since p0 ends at 7.5 and p1 could not reach
+// the rest.
 //
 // A group that holds an infinity or a NaN gets the scale 255 (not a number).
 #pragma once
@@ -32,8 +41,10 @@ constexpr int kMxGroup = 32;
 constexpr int kMxPieceBytes = 24;     // 32 values of 6 bits
 constexpr int kMxPairBytes = 48;      // p0, p1 of a group
 constexpr int kMxThirdBytes = 32;     // p2 of a group, padded to whole 16 bytes
-// The least scale byte of p0: the last piece's, 4 or 8 below, is at least 1.
-constexpr int kMxMinScalePair = 5, kMxMinScaleThird = 9;
+constexpr int kMxTokenShift = 4;      // p1's power of two below p0's
+constexpr int kMxInterShift = 5;
+// The least scale byte of p0: the last piece's, 8 or 5 below, is at least 1.
+constexpr int kMxMinToken = 9, kMxMinInter = 6;
 
 // 32 floats over 2^x to E2M3, nearest even.  The instruction takes the even
 // and the odd values apart, and writes its result while it still reads its
@@ -58,8 +69,8 @@ __device__ __forceinline__ float mx_pow2(int biased) {
   return __uint_as_float(uint32_t(biased) << 23);
 }
 
-// The scale byte of a group and its first two pieces; v is left with the rest.
-// With THIRD also p2 (zeros where no value stands out, and then false).
+// The scale byte of a group and its pieces; v is left with the rest.  THIRD: a
+// token's, with p2 (zeros where no value stands out, and then false).
 template <bool THIRD>
 __device__ __forceinline__ bool mx_split(float (&v)[32], int& scale, u32x6& p0, u32x6& p1,
                                          u32x6& p2) {
@@ -67,7 +78,9 @@ __device__ __forceinline__ bool mx_split(float (&v)[32], int& scale, u32x6& p0, 
 #pragma unroll
   for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
   const int e = int(top >> 23);
-  const int s = max(e - 2, THIRD ? kMxMinScaleThird : kMxMinScalePair);
+  // intermediates: 7.75 = 4 * 1.9375, the mantissa 0xf8 over 8 bits
+  const int up = !THIRD && (top & 0x7fffffu) >= 0x780000u ? 1 : 0;
+  const int s = max(e - 2 + up, THIRD ? kMxMinToken : kMxMinInter);
   bool peak = false;
   if constexpr (THIRD) {
     // in units of 2^s the squares neither overflow nor vanish
@@ -86,7 +99,7 @@ __device__ __forceinline__ bool mx_split(float (&v)[32], int& scale, u32x6& p0, 
   f32x32 b = mx_from_fp6(p0, f);
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] -= b[i];
-  const float f1 = mx_pow2(s - 4);
+  const float f1 = mx_pow2(s - (THIRD ? kMxTokenShift : kMxInterShift));
   p1 = mx_to_fp6(v, f1);
   p2 = u32x6{0, 0, 0, 0, 0, 0};
   if constexpr (THIRD) {
@@ -94,7 +107,7 @@ __device__ __forceinline__ bool mx_split(float (&v)[32], int& scale, u32x6& p0, 
       b = mx_from_fp6(p1, f1);
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] -= b[i];
-      p2 = mx_to_fp6(v, mx_pow2(s - 8));
+      p2 = mx_to_fp6(v, mx_pow2(s - 2 * kMxTokenShift));
     }
   }
   scale = e == 255 ? 255 : s;

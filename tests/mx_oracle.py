@@ -56,9 +56,13 @@ def ffn(x, gate, up, down):
     """(y, bound): the expert on rows x [m, hidden] in 64 bits, and how far
     the kernel's fp32 value may be off before it is rounded to bf16.
 
-    An activation is held to 2^-10 of its group's largest (2^-9 of itself where
-    it is among the largest: less than 2^-9 of the largest), an intermediate to
-    2^-9 of its group's largest; the sums are fp32, off by at most one rounding
+    An activation is held to 2^-10 of its group's largest: it is bf16, and exact
+    in two pieces where it is an eighth of the largest and more.  An intermediate
+    is held to 2^-8 of its group's largest M: with 2^e the group's unit and M in
+    [3.875, 7.75) 2^e, the second piece (unit 2^(e-5), steps of 1/8, 1/4, 1/2 up
+    to 7.5) leaves 2^-10, 2^-9 and 2^-8 2^e of rests of up to 1/16, 1/8 and 15/64
+    2^e, and 1/4 - 15/64 = 2^-6 2^e of a rest of 1/4 2^e, which only a value of
+    4 2^e and more leaves, so that M is 4 2^e too.  The sums are fp32, off by at most one rounding
     for each of the reduction's 128-wide steps and pieces and the waves' sums
     (under 2^-16 of the sum of magnitudes); silu's derivative is below 1.1, its
     fp32 value is off by under 2^-20."""
@@ -70,5 +74,5 @@ def ffn(x, gate, up, down):
         sg = g / (1 + np.exp(-g))
     h = sg * u
     dh = 1.1 * dg * (np.abs(u) + du) + np.abs(sg) * du + 2.0 ** -20 * np.abs(h)
-    ah = dh + 2.0 ** -9 * group_max(np.abs(h) + dh) + 2.0 ** -16 * np.abs(h)
+    ah = dh + 2.0 ** -8 * group_max(np.abs(h) + dh) + 2.0 ** -16 * np.abs(h)
     return h @ down.T, ah @ np.abs(down).T

@@ -218,6 +218,35 @@ def test_seam_dropped_absent_and_repeated_ids(n):
     assert torch.equal(y[:, 0], y[:, 1])
 
 
+@pytest.mark.parametrize("pin", ["0", "1"])
+@pytest.mark.parametrize("hidden,inter,experts,n,k", [
+    (128, 128, 2, 1, 1), (128, 256, 3, 50, 2), (256, 128, 3, 200, 2), (640, 384, 2, 129, 1),
+    (1024, 512, 4, 140, 2), (384, 640, 2, 300, 2), (4096, 1536, 2, 67, 2), (8192, 128, 1, 20, 1),
+    (128, 8192, 1, 20, 1)])
+def test_tile_forms(monkeypatch, pin, hidden, inter, experts, n, k):
+    """Both forms of the products at both sides of the rule between them: tiles
+    of 16 and of 128 rows, with rows that end inside a tile, features that end
+    inside a block, dropped ids and an expert without a slot."""
+    monkeypatch.setenv("PMOE_MX_TILE", pin)
+    rng = np.random.default_rng(hidden + n)
+    L = Layer(hidden, inter, experts, perm=True)
+    x = tokens(rng, n, hidden)
+    inds = rng.integers(0, experts, (n, k)).astype(np.int32)
+    inds[rng.random((n, k)) < 0.05] = -1
+    table = L.table.clone()
+    if experts > 2:
+        table[1] = -1
+        inds_ref = np.where(inds == 1, -1, inds)
+    else:
+        inds_ref = inds
+    y = K.switch_glu(L.g, L.slab.buf, table, experts, x, torch.from_numpy(inds).to(DEV))
+    ref, b = L.seam(x.double().cpu().numpy(), inds_ref)
+    check(y, ref, b)
+    assert (y.cpu()[torch.from_numpy(inds_ref < 0)].view(torch.int16) == 0).all()
+    assert torch.equal(y, K.switch_glu(L.g, L.slab.buf, table, experts, x,
+                                       torch.from_numpy(inds).to(DEV)))
+
+
 def combined(L, x, inds, w, gate=None):
     y, b = L.seam(x, inds)
     out = (y * w[..., None]).sum(1)
