@@ -53,6 +53,7 @@ struct MoeWs {
   uint8_t *xpair = nullptr, *xthird = nullptr, *xscale = nullptr;
   uint16_t* xsteps = nullptr;
   uint8_t *hpair = nullptr, *hscale = nullptr;
+  uint8_t* yscale = nullptr;  // of the slot outputs that the combine reads
 };
 
 struct Carver {
@@ -88,14 +89,15 @@ size_t carve(const pmoe_geom* g, int n, int k, int shared, int n_experts, void* 
   t.tiles = c.take<int4>(t.max_tiles);
   t.n_tiles = c.take<int32_t>(1);
   if (mx) {
-    const size_t xg = size_t(n) * (g->hidden / kMxGroup), hg = rows * (g->inter / kMxGroup);
-    t.xpair = c.take<uint8_t>(xg * kMxPairBytes);
-    t.xthird = c.take<uint8_t>(xg * kMxThirdBytes);
-    t.xscale = c.take<uint8_t>(xg);
+    const size_t xs = size_t(n) * mx_steps(g->hidden), hs = rows * mx_steps(g->inter);
+    t.xpair = c.take<uint8_t>(xs * kMxStepPair);
+    t.xthird = c.take<uint8_t>(xs * kMxStepThird);
+    t.xscale = c.take<uint8_t>(size_t(n) * mx_scale_row(g->hidden));
     t.xsteps = c.take<uint16_t>(size_t(n) * 4);
-    t.hpair = c.take<uint8_t>(hg * kMxPairBytes);
-    t.hscale = c.take<uint8_t>(hg);
-    t.y = reinterpret_cast<float*>(c.take<uint16_t>(rows * g->hidden));  // bf16 rows only
+    t.hpair = c.take<uint8_t>(hs * kMxStepPair);
+    t.hscale = c.take<uint8_t>(rows * mx_scale_row(g->inter));
+    t.y = reinterpret_cast<float*>(c.take<uint16_t>(rows * g->hidden));
+    t.yscale = c.take<uint8_t>(rows * (g->hidden / kMxGroup));
   } else {
     t.h = c.take<uint16_t>(rows * g->inter);
     t.y = c.take<float>(rows * g->hidden);
@@ -199,9 +201,9 @@ __global__ __launch_bounds__(256) void combine_bf16_kernel(const uint16_t* __res
 __global__ __launch_bounds__(256) void zero_dropped_rows_kernel(const int32_t* __restrict__ inv,
                                                                 int rows, int d,
                                                                 uint16_t* __restrict__ y) {
-  const int r = blockIdx.y;
+  const int r = blockIdx.x;
   if (r >= rows || inv[r] >= 0) return;
-  for (int i = blockIdx.x * 256 + threadIdx.x; i < d; i += gridDim.x * 256) y[size_t(r) * d + i] = 0;
+  for (int i = threadIdx.x; i < d; i += 256) y[size_t(r) * d + i] = 0;
 }
 
 int check_geom(const pmoe_geom* g, const void* slab) {
@@ -315,6 +317,7 @@ int run_experts(const pmoe_geom* g, const uint8_t* slab, const int32_t* table, i
     p.max_tiles = rows / tm + std::min(rows, n_ids) + 1;
     p.xpair = w.xpair, p.xthird = w.xthird, p.xscale = w.xscale, p.xsteps = w.xsteps;
     p.hpair = w.hpair, p.hscale = w.hscale, p.y = static_cast<uint16_t*>(y);
+    p.yscale = y == w.y ? w.yscale : nullptr;
     return mx_experts(p, st);
   }
   const bool stream = stream_wanted(g, slab, n, kk, n_experts, n_ids);
@@ -542,6 +545,9 @@ int experts_and_combine(const pmoe_geom* g, const uint8_t* slab, const int32_t* 
     if (rc) return rc;
     sl = w.shared_logit;
   }
+  if (is_mx(g))
+    return mx_combine(reinterpret_cast<const uint16_t*>(w.y), w.yscale, wts, w.inv, sl, n, k, kk,
+                      g->hidden, out, st);
   dim3 grid((g->hidden / 8 + 255) / 256, n);
   ProfScope prof_scope(K_COMBINE, st);
   combine_kernel<<<grid, 256, 0, st>>>(reinterpret_cast<const uint16_t*>(w.y), wts, w.inv, sl,
@@ -619,7 +625,7 @@ extern "C" int pmoe_switch_glu(const pmoe_geom* g, const void* slab, const int32
   rc = pmoe::run_experts(g, static_cast<const uint8_t*>(slab), table, n_experts, -1,
                          static_cast<const uint16_t*>(x), inds, n, k, k, n * k, w, y, 0, st);
   if (rc) return rc;
-  dim3 grid(1, n * k);
+  dim3 grid(n * k);
   pmoe::zero_dropped_rows_kernel<<<grid, 256, 0, st>>>(w.inv, n * k, g->hidden,
                                                        static_cast<uint16_t*>(y));
   PMOE_LAUNCH_CHECK("zero_dropped_rows_kernel");

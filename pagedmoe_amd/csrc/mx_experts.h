@@ -18,13 +18,14 @@ struct MxArgs {
   const int32_t* n_tiles;
   const int32_t* order;    // sorted position -> flat row
   int kk, features, cols;
-  const uint8_t* pair;     // [rows, cols / 32, 48]
-  const uint8_t* third;    // [rows, cols / 32, 32]
-  const uint8_t* ascale;   // [rows, cols / 32]
+  const uint8_t* pair;     // rows of pieces (mx_pieces.h)
+  const uint8_t* third;
+  const uint8_t* ascale;   // their scales
   const uint16_t* asteps;  // [rows, 4]: bit s: step s of 128 has a third piece
-  uint8_t* hpair;          // gate/up out: [sorted row, features / 32, 48]
+  uint8_t* hpair;          // gate/up out, by sorted row
   uint8_t* hscale;
-  uint16_t* y;             // down out: bf16 [flat row, features]
+  uint16_t* y;             // down out: [flat row, features], bf16 or fp16 under yscale
+  uint8_t* yscale;         // [flat row, features / 32]
 };
 
 struct MxPlan {
@@ -41,7 +42,8 @@ struct MxPlan {
   uint8_t *xpair, *xthird, *xscale;
   uint16_t* xsteps;  // [n, 4]
   uint8_t *hpair, *hscale;
-  uint16_t* y;  // bf16 [n * kk, hidden]
+  uint16_t* y;      // [n * kk, hidden]: bf16, or fp16 under yscale where that is not null
+  uint8_t* yscale;  // [n * kk, hidden / 32]
 };
 
 // Rows of the dispatch's tiles for such a call, and the fewest that any has.
@@ -50,5 +52,9 @@ int mx_min_tile_rows();
 // Split, gate/up, down over the dispatch's tiles; rows whose expert is not
 // resident come out zero.
 int mx_experts(const MxPlan& p, hipStream_t st);
+// out[n] = sum over columns in order of weight * y (+ the shared column's).
+int mx_combine(const uint16_t* y, const uint8_t* yscale, const float* w, const int32_t* inv,
+               const float* shared_logit, int n, int k, int kk, int d, uint16_t* out,
+               hipStream_t st);
 
 }  // namespace pmoe

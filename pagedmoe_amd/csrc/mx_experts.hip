@@ -10,7 +10,10 @@
 //
 // An activation that is infinite or NaN, or an intermediate that leaves fp32,
 // makes the outputs of its row NaN.
+#include <hip/hip_fp16.h>
 #include <stdlib.h>
+
+#include <type_traits>
 
 #include "mx_experts.h"
 #include "mx_pieces.h"
@@ -26,6 +29,13 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kFp4 = 4, kFp6 = 2;  // operand formats of the scaled MFMA
 
+__device__ __forceinline__ const uint8_t* uniform_ptr(const uint8_t* p) {
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(uint32_t(v));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(uint32_t(v >> 32));
+  return reinterpret_cast<const uint8_t*>(uint64_t(lo) | uint64_t(hi) << 32);
+}
+
 // acc += W (16 rows x 128) times a piece of 16 activation rows; sw, sp: the
 // lane's scale bytes.
 __device__ __forceinline__ void mx_mma(f32x4& acc, const uint4& w, int sw, const uint32_t (&p)[6],
@@ -35,12 +45,87 @@ __device__ __forceinline__ void mx_mma(f32x4& acc, const uint4& w, int sw, const
   acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, kFp4, kFp6, 0, sw, 0, sp);
 }
 
+// The same with a third piece, in the weights' format.
+__device__ __forceinline__ void mx_mma_third(f32x4& acc, const uint4& w, int sw, const uint4& p,
+                                             int sp) {
+  const i32x8 a = {int(w.x), int(w.y), int(w.z), int(w.w), 0, 0, 0, 0};
+  const i32x8 b = {int(p.x), int(p.y), int(p.z), int(p.w), 0, 0, 0, 0};
+  acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, kFp4, kFp4, 0, sw, 0,
+                                                         sp - kMxThirdShift);
+}
+
+// ---------------------------------------------------------------- slot outputs
+//
+// Outputs that go on to the combine are held in 16 bits: fp16 under a power of
+// two for each 32 features of a row (scale byte s: value 2^(s - 127)), which
+// leaves 2^-12 of a value where bf16 would leave 2^-9.  The largest of the 32 is
+// brought into [2^14, 2^15).  255: an infinity or a NaN among them.
+
+__device__ __forceinline__ int half_scale(uint32_t top) {
+  const int e = int(top >> 23);
+  return e == 255 ? 255 : max(e - 14, 1);
+}
+
+__device__ __forceinline__ uint16_t half_of(float v, int s) {
+  return __half_as_ushort(__float2half_rn(v * mx_pow2(254 - min(s, 253))));
+}
+
+__device__ __forceinline__ float half_unit(int s) {
+  return s == 255 ? __uint_as_float(0x7fc00000u) : mx_pow2(s);
+}
+
+// The largest over the lane's half of the wave (32 lanes).
+__device__ __forceinline__ uint32_t half_wave_max(uint32_t v) {
+  auto other = [&](auto d) {
+    return uint32_t(__float_as_int(xor_lane<decltype(d)::value>(__int_as_float(int(v)))));
+  };
+  v = max(v, other(std::integral_constant<int, 16>{}));
+  v = max(v, other(std::integral_constant<int, 8>{}));
+  v = max(v, other(std::integral_constant<int, 4>{}));
+  v = max(v, other(std::integral_constant<int, 2>{}));
+  v = max(v, other(std::integral_constant<int, 1>{}));
+  return v;
+}
+
+// out[n] = bf16(fma over k of weight * y, then the shared expert's times 1 or
+// sigmoid(shared_logit[n])), in column order; 8 features a thread.
+__global__ __launch_bounds__(256) void mx_combine_kernel(
+    const uint16_t* __restrict__ y, const uint8_t* __restrict__ yscale,
+    const float* __restrict__ w, const int32_t* __restrict__ inv,
+    const float* __restrict__ shared_logit, int k, int kk, int d, int blocks_row,
+    uint16_t* __restrict__ out) {
+  const int n = blockIdx.x / blocks_row;
+  const int d0 = ((blockIdx.x - n * blocks_row) * 256 + threadIdx.x) * 8;
+  if (d0 >= d) return;
+  float a[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+  for (int c = 0; c < kk; ++c) {
+    const size_t r = size_t(n) * kk + c;
+    if (inv[r] < 0) continue;  // dropped id: contributes nothing
+    float wt = c < k ? w[size_t(n) * k + c] : shared_logit ? psigmoid(shared_logit[n]) : 1.0f;
+    const float unit = half_unit(yscale[r * (d / kMxGroup) + d0 / kMxGroup]);
+    const uint4 v = *reinterpret_cast<const uint4*>(y + r * d + d0);
+    const uint32_t p[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[2 * i] = __builtin_fmaf(
+          wt, __half2float(__ushort_as_half(uint16_t(p[i]))) * unit, a[2 * i]);
+      a[2 * i + 1] = __builtin_fmaf(
+          wt, __half2float(__ushort_as_half(uint16_t(p[i] >> 16))) * unit, a[2 * i + 1]);
+    }
+  }
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = uint32_t(f2bf(a[2 * i])) | uint32_t(f2bf(a[2 * i + 1])) << 16;
+  *reinterpret_cast<uint4*>(out + size_t(n) * d + d0) = make_uint4(o[0], o[1], o[2], o[3]);
+}
+
 // ---------------------------------------------------------------- activations
 
 // One lane a group: x bf16 [n, d] into pieces, scales and each token's mask of
 // the 128-wide steps that hold a third piece (16 bits a wave, 4 waves a token).
 __global__ __launch_bounds__(256) void mx_split_kernel(const uint16_t* __restrict__ x, int n,
-                                                       int groups, uint8_t* __restrict__ pair,
+                                                       int groups, int steps128, int scale_row,
+                                                       uint8_t* __restrict__ pair,
                                                        uint8_t* __restrict__ third,
                                                        uint8_t* __restrict__ scales,
                                                        uint16_t* __restrict__ steps) {
@@ -48,8 +133,9 @@ __global__ __launch_bounds__(256) void mx_split_kernel(const uint16_t* __restric
   const int g = threadIdx.x;
   bool peak = false;
   if (g < groups) {
-    const size_t at = size_t(token) * groups + g;
-    const uint4* src = reinterpret_cast<const uint4*>(x + at * kMxGroup);
+    const size_t row = size_t(token) * steps128;
+    const uint4* src =
+        reinterpret_cast<const uint4*>(x + (size_t(token) * groups + g) * kMxGroup);
     float v[32];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -60,11 +146,12 @@ __global__ __launch_bounds__(256) void mx_split_kernel(const uint16_t* __restric
         v[8 * i + 2 * j] = bf16lo(w[j]), v[8 * i + 2 * j + 1] = bf16hi(w[j]);
     }
     int s;
-    u32x6 p0, p1, p2;
+    u32x6 p0, p1;
+    uint4 p2;
     peak = mx_split<true>(v, s, p0, p1, p2);
-    mx_store_pair(pair + at * kMxPairBytes, p0, p1);
-    mx_store_third(third + at * kMxThirdBytes, p2);
-    scales[at] = uint8_t(s);
+    mx_store_pair(pair + row * kMxStepPair, g, p0, p1);
+    mx_store_third(third + row * kMxStepThird, g, p2);
+    scales[size_t(token) * scale_row + mx_scale_at(g)] = uint8_t(s);
   }
   const uint64_t m = __ballot(peak);
   if ((threadIdx.x & 63) == 0) {
@@ -86,7 +173,7 @@ constexpr int kMaxWaves = 8;
 // and the same 32 up features).  The waves share the reduction: wave w takes
 // steps w, w + waves, ... of 512, all loads of a step in flight at once, and
 // the partial sums meet in LDS.  FULL: the reduction is whole steps.
-template <bool DUAL, bool FULL>
+template <bool DUAL, bool FULL, bool HALF>
 __global__ __launch_bounds__(64 * kMaxWaves) void mx_small_kernel(const MxArgs a) {
   constexpr int NF = DUAL ? 4 : 2;  // 16-feature tiles: gate, gate, up, up
   __shared__ float s_red[kMaxWaves][NF * 4][64];
@@ -103,9 +190,11 @@ __global__ __launch_bounds__(64 * kMaxWaves) void mx_small_kernel(const MxArgs a
   const int lane = threadIdx.x & 63;
   if (tile.x < 0) {  // not resident: exact zero rows
     if constexpr (!DUAL) {
-      for (int i = threadIdx.x; i < m * kSmallCols; i += blockDim.x)
-        a.y[size_t(a.order[p0 + i / kSmallCols]) * a.features + fb * kSmallCols +
-            i % kSmallCols] = 0;
+      for (int i = threadIdx.x; i < m * kSmallCols; i += blockDim.x) {
+        const size_t flat = a.order[p0 + i / kSmallCols];
+        a.y[flat * a.features + fb * kSmallCols + i % kSmallCols] = 0;
+        if (HALF && i % kSmallCols == 0) a.yscale[flat * fblocks + fb] = 1;
+      }
     }
     return;
   }
@@ -122,9 +211,10 @@ __global__ __launch_bounds__(64 * kMaxWaves) void mx_small_kernel(const MxArgs a
     wrow[f] = base + (f < 2 ? a.w0 : a.w1) + row * size_t(a.cols / 2);
     srow[f] = base + (f < 2 ? a.s0 : a.s1) + row * size_t(groups);
   }
-  const uint8_t* pair = a.pair + arow * groups * kMxPairBytes;
-  const uint8_t* third = DUAL ? a.third + arow * groups * kMxThirdBytes : nullptr;
-  const uint8_t* ascale = a.ascale + arow * groups;
+  const size_t asteps = arow * mx_steps(a.cols);
+  const uint8_t* pair = a.pair + asteps * kMxStepPair;
+  const uint8_t* third = DUAL ? a.third + asteps * kMxStepThird : nullptr;
+  const uint8_t* ascale = a.ascale + arow * mx_scale_row(a.cols);
   f32x4 acc[NF];
 #pragma unroll
   for (int f = 0; f < NF; ++f) acc[f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -148,9 +238,10 @@ __global__ __launch_bounds__(64 * kMaxWaves) void mx_small_kernel(const MxArgs a
       const int g = 16 * j + 4 * i + q;
       const bool in = FULL || g < groups;
       const int gc = in ? g : 0;
-      const uint4* src = reinterpret_cast<const uint4*>(pair + size_t(gc) * kMxPairBytes);
-      const uint4 c0 = src[0], c1 = src[1], c2 = src[2];
-      const int sa = in ? ascale[gc] : 127;
+      const uint4* src =
+          reinterpret_cast<const uint4*>(pair + (gc >> 2) * kMxStepPair + (gc & 3) * 16);
+      const uint4 c0 = src[0], c1 = src[kMxChunk / 16], c2 = src[2 * kMxChunk / 16];
+      const int sa = in ? ascale[mx_scale_at(gc)] : 127;
       const uint32_t b0[6] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y};
       const uint32_t b1[6] = {c1.z, c1.w, c2.x, c2.y, c2.z, c2.w};
 #pragma unroll
@@ -159,11 +250,10 @@ __global__ __launch_bounds__(64 * kMaxWaves) void mx_small_kernel(const MxArgs a
       for (int f = 0; f < NF; ++f)
         mx_mma(acc[f], w[f][i], sw[f][i], b1, sa - (DUAL ? kMxTokenShift : kMxInterShift));
       if constexpr (DUAL) {
-        const uint4* s3 = reinterpret_cast<const uint4*>(third + size_t(gc) * kMxThirdBytes);
-        const uint4 d0 = s3[0], d1 = s3[1];
-        const uint32_t b2[6] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y};
+        const uint4 d = *reinterpret_cast<const uint4*>(third + (gc >> 2) * kMxStepThird +
+                                                        (gc & 3) * 16);
 #pragma unroll
-        for (int f = 0; f < NF; ++f) mx_mma(acc[f], w[f][i], sw[f][i], b2, sa - 2 * kMxTokenShift);
+        for (int f = 0; f < NF; ++f) mx_mma_third(acc[f], w[f][i], sw[f][i], d, sa);
       }
     }
   }
@@ -173,8 +263,9 @@ __global__ __launch_bounds__(64 * kMaxWaves) void mx_small_kernel(const MxArgs a
     for (int i = 0; i < 4; ++i) s_red[wave][4 * f + i][lane] = acc[f][i];
   __syncthreads();
   // feature c of row s_r: accumulator c % 4 of lane 16 (c % 16 / 4) + row
-  for (int i = threadIdx.x; i < m * kSmallCols; i += blockDim.x) {
+  for (int i = threadIdx.x; i < kSmallRows * kSmallCols; i += blockDim.x) {
     const int row = i / kSmallCols, c = i % kSmallCols;
+    if (row >= m) break;  // whole halves of a wave
     const int src = (c & 15) / 4 * 16 + row;
     float v = 0.0f, u = 0.0f;
     for (int k = 0; k < waves; ++k) {
@@ -183,8 +274,17 @@ __global__ __launch_bounds__(64 * kMaxWaves) void mx_small_kernel(const MxArgs a
     }
     if constexpr (DUAL)
       s_h[row][c] = silu_fast(v) * u;
-    else
-      a.y[size_t(a.order[p0 + row]) * a.features + fb * kSmallCols + c] = f2bf(v);
+    else {
+      const size_t flat = a.order[p0 + row];
+      uint16_t* y = a.y + flat * a.features + fb * kSmallCols + c;
+      if constexpr (HALF) {
+        const int sc = half_scale(half_wave_max(__float_as_uint(v) & 0x7fffffffu));
+        *y = half_of(v, sc);
+        if (c == 0) a.yscale[flat * fblocks + fb] = uint8_t(sc);
+      } else {
+        *y = f2bf(v);
+      }
+    }
   }
   if constexpr (DUAL) {
     __syncthreads();
@@ -193,16 +293,17 @@ __global__ __launch_bounds__(64 * kMaxWaves) void mx_small_kernel(const MxArgs a
 #pragma unroll
       for (int c = 0; c < 32; ++c) v[c] = s_h[threadIdx.x][c];
       int s;
-      u32x6 h0, h1, h2;
-      mx_split<false>(v, s, h0, h1, h2);
-      const size_t at = size_t(p0 + threadIdx.x) * fblocks + fb;
-      mx_store_pair(a.hpair + at * kMxPairBytes, h0, h1);
-      a.hscale[at] = uint8_t(s);
+      u32x6 h0, h1;
+      uint4 none;
+      mx_split<false>(v, s, h0, h1, none);
+      const size_t row = size_t(p0 + threadIdx.x) * mx_steps(a.features);
+      mx_store_pair(a.hpair + row * kMxStepPair, fb, h0, h1);
+      a.hscale[size_t(p0 + threadIdx.x) * mx_scale_row(a.features) + mx_scale_at(fb)] = uint8_t(s);
     }
   }
 }
 
-template <bool DUAL>
+template <bool DUAL, bool HALF>
 int launch_small(const MxArgs& a, int max_tiles, hipStream_t st) {
   const int steps = (a.cols + kStep - 1) / kStep;
   const int rounds = (steps + kMaxWaves - 1) / kMaxWaves;
@@ -211,9 +312,9 @@ int launch_small(const MxArgs& a, int max_tiles, hipStream_t st) {
   PMOE_REQUIRE(blocks < (int64_t(1) << 31) / 1, "experts: too many tiles for one call");
   ProfScope prof_scope(DUAL ? K_MX_GATEUP : K_MX_DOWN, st);
   if (a.cols % kStep == 0)
-    mx_small_kernel<DUAL, true><<<unsigned(blocks), 64 * waves, 0, st>>>(a);
+    mx_small_kernel<DUAL, true, HALF><<<unsigned(blocks), 64 * waves, 0, st>>>(a);
   else
-    mx_small_kernel<DUAL, false><<<unsigned(blocks), 64 * waves, 0, st>>>(a);
+    mx_small_kernel<DUAL, false, HALF><<<unsigned(blocks), 64 * waves, 0, st>>>(a);
   PMOE_LAUNCH_CHECK("mx_small_kernel");
   return PMOE_OK;
 }
@@ -225,53 +326,51 @@ constexpr int kTileCols = 512;    // weight rows a block (DUAL: 256 gate, 256 up
 constexpr int kTileWaves = 8;     // 2 halves of the rows x 4 quarters of the weights
 constexpr int kActBytes = 8 * 3 * 1024;             // 8 row tiles x 3 chunks a lane
 constexpr int kWeightBytes = kTileCols / 16 * 1024;  // 32 row tiles x 1 chunk a lane
-constexpr int kActScaleBytes = kTileWaves * 256;
-constexpr int kWeightScaleBytes = kTileWaves * 256;
-constexpr int kStageBytes = kActBytes + kWeightBytes + kActScaleBytes + kWeightScaleBytes;
-constexpr int kTileLds = 2 * kStageBytes;
+constexpr int kThirdBytes = 8 * 1024;                // 8 row tiles x 1 chunk a lane
+constexpr int kStageBytes = kActBytes + kWeightBytes + kThirdBytes;
+// 16 scale bytes a row, of four steps
+constexpr int kActScaleBytes = kTileRows * kMxScaleBlock;
+constexpr int kScaleBytes = kActScaleBytes + kTileCols * kMxScaleBlock;
+constexpr int kTileLds = 2 * (kStageBytes + kScaleBytes);
 
-// 16 bytes (4 bytes) a lane from p to LDS [lds, lds + 1024) ([.., + 256)), lane l
-// at 16 l (4 l).
-__device__ __forceinline__ void dma16(uint32_t lds, const uint8_t* p) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+// 16 bytes (4 bytes) a lane from base + voff to LDS [lds, lds + 1024) ([.., +
+// 256)), lane l at 16 l (4 l).  base and lds are the wave's.
+__device__ __forceinline__ void dma16(uint32_t lds, uint32_t voff, const uint8_t* base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                :
-               : "s"(lds), "v"(p)
+               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(uniform_ptr(base))
                : "memory");
 }
 
-__device__ __forceinline__ void dma4(uint32_t lds, const uint8_t* p) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+__device__ __forceinline__ void dma4(uint32_t lds, uint32_t voff, const uint8_t* base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
                :
-               : "s"(lds), "v"(p)
+               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(uniform_ptr(base))
                : "memory");
 }
 
-// The steps of a tile's reduction, in order: every 128-wide step with the first
-// two pieces, then, for tokens, those steps in which a row of the tile has a
-// third piece.
+// The steps of a tile's reduction: s done of n.
 struct Steps {
   int s, n;
-  uint64_t left;
-  __device__ __forceinline__ bool third() const { return s >= n; }
-  __device__ __forceinline__ int step() const {
-    return third() ? __builtin_ctzll(left) : s;
-  }
-  __device__ __forceinline__ void next() {
-    if (third())
-      left &= left - 1;
-    else
-      ++s;
-  }
-  __device__ __forceinline__ bool done() const { return third() && left == 0; }
+  // whether the step's scales are not in the block of the step before
+  __device__ __forceinline__ bool fresh() const { return s % kMxScaleSteps == 0; }
+  __device__ __forceinline__ bool done() const { return s >= n; }
 };
 
 // One tile of at most 128 rows of an expert times 512 weight rows (DUAL: 256
 // gate and the same 256 up features).  Each wave holds 64 rows times 128 weight
-// rows in its accumulators.  A step of 128 goes from memory straight into LDS
-// in the order in which the lanes read it back, 16 bytes a lane, so that no
-// read has a bank conflict; the next step's loads are in flight while this
-// one's products run.
-template <bool DUAL>
+// rows in its accumulators.  A step of 128 goes from memory straight into LDS,
+// 16 rows of 64 bytes an instruction: lane l fetches chunk (l & 3) ^ (l >> 4) of
+// row l >> 2, so that four lanes side by side fetch one 64-byte stretch (lanes
+// in the products' own order, 16 rows side by side, cost the cache four times
+// the accesses and bound the kernel) and the 16 lanes that read one chunk of 16
+// rows back meet 16 different banks of 16 bytes.  The next step's loads are in
+// flight while this one's products run.
+// Scales come 16 bytes a row, those of four steps.  BLOCKS: the reduction is
+// whole stretches of 512, so that the weights' lie on 16 bytes too; otherwise
+// theirs are fetched 4 bytes a row for each step (those fetches alone took a
+// sixth of the kernel's time where every step did so).
+template <bool DUAL, bool BLOCKS, bool HALF>
 __global__ __launch_bounds__(64 * kTileWaves, 2) void mx_tile_kernel(const MxArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kTileLds];
   __shared__ unsigned long long s_third;
@@ -293,9 +392,12 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void mx_tile_kernel(const MxArg
   if (tile.x < 0) {  // not resident: exact zero rows
     if constexpr (!DUAL) {
       const int cols = min(kCols, a.features - fb * kCols);
-      for (int row = wave; row < m; row += kTileWaves)
-        for (int c = lane; c < cols; c += 64)
-          a.y[size_t(a.order[p0 + row]) * a.features + fb * kCols + c] = 0;
+      for (int row = wave; row < m; row += kTileWaves) {
+        const size_t flat = a.order[p0 + row];
+        for (int c = lane; c < cols; c += 64) a.y[flat * a.features + fb * kCols + c] = 0;
+        if (HALF && lane < cols / kMxGroup)
+          a.yscale[(flat * a.features + fb * kCols) / kMxGroup + lane] = 1;
+      }
     }
     return;
   }
@@ -303,30 +405,36 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void mx_tile_kernel(const MxArg
   const int groups = a.cols / kMxGroup;
   const uint8_t* base = a.slab + size_t(tile.x) * size_t(a.expert_bytes);
 
-  // What this wave loads each step: row tile `wave` of the activations (and its
-  // scales), weight tiles 4 wave .. + 3 and the scales of those 64 rows.
-  const int lrow = 16 * wave + r;
-  const int lpos = p0 + (lrow < m ? lrow : 0);
-  const size_t arow = DUAL ? size_t(a.order[lpos] / a.kk) : size_t(lpos);
-  const uint8_t* pair = a.pair + (arow * groups + q) * kMxPairBytes;
-  const uint8_t* third = DUAL ? a.third + (arow * groups + q) * kMxThirdBytes : nullptr;
-  const uint8_t* ascale = a.ascale + arow * groups;
-  // weight row w of the block: its gate (0..255) or up feature; rows past the
-  // projection load its last ones and are not used
-  const auto weight_row = [&](int w) {
-    const int f = fb * kCols + (DUAL ? w & (kCols - 1) : w);
-    return size_t(min(f, a.features - 1));
+  // What this wave loads each step: row tile `wave` of the activations and
+  // weight tiles 4 wave .. + 3, now and then their scales.  Offsets from the
+  // wave's own bases; a tile's intermediate rows follow each other, tokens lie
+  // anywhere in less than 4 GiB (mx_tile_rows).
+  const int lr = lane >> 2, lq = (lane & 3) ^ (lane >> 4);
+  const int steps = groups / kMxStepGroups;
+  const auto act_row = [&](int row) {
+    const int k = row < m ? row : 0;
+    return uint32_t(DUAL ? a.order[p0 + k] / a.kk : k);
+  };
+  const size_t arow0 = DUAL ? 0 : size_t(p0);
+  const uint8_t* apair = a.pair + arow0 * steps * kMxStepPair;
+  const uint8_t* ascale = a.ascale + arow0 * mx_scale_row(a.cols);
+  const uint32_t arow = act_row(16 * wave + lr) * uint32_t(steps);
+  const uint32_t pair_off = arow * kMxStepPair + lq * 16;
+  const uint32_t third_off = arow * kMxStepThird + lq * 16;
+  const uint32_t ascale_off = act_row(16 * wave + r) * uint32_t(mx_scale_row(a.cols));
+  // the block's weight tile i: its gate (0..15) or up features; tiles past the
+  // projection load its last one and are not used
+  const auto tile_row = [&](int i) {
+    return min(fb * kCols + (DUAL ? 16 * i & (kCols - 1) : 16 * i), a.features - 16);
   };
   const bool second = DUAL && wave >= kTileWaves / 2;
   const uint8_t* wbase = base + (second ? a.w1 : a.w0);
-  const uint8_t* wsrc[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    wsrc[i] = wbase + weight_row(64 * wave + 16 * i + r) * size_t(a.cols / 2) + q * 16;
-  const uint8_t* wscale =
-      base + (second ? a.s1 : a.s0) + weight_row(64 * wave + lane) * size_t(groups);
+  const uint8_t* wscale = base + (second ? a.s1 : a.s0);
+  const uint32_t w_off = uint32_t(lr) * uint32_t(a.cols / 2) + lq * 16;
+  const uint32_t wscale_off = uint32_t(tile_row(4 * wave + q) + r) * uint32_t(groups);
 
-  Steps todo{0, groups / 4, 0};
+  Steps todo{0, steps};
+  uint64_t thirds = 0;  // bit s: a row of the tile has a third piece in step s
   if constexpr (DUAL) {
     if (threadIdx.x == 0) s_third = 0;
     __syncthreads();
@@ -338,29 +446,42 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void mx_tile_kernel(const MxArg
     const uint64_t v = s_third;
     const uint32_t lo = __builtin_amdgcn_readfirstlane(uint32_t(v));
     const uint32_t hi = __builtin_amdgcn_readfirstlane(uint32_t(v >> 32));
-    todo.left = uint64_t(lo) | uint64_t(hi) << 32;
+    thirds = uint64_t(lo) | uint64_t(hi) << 32;
   }
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(
       uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds)));
-  const auto issue = [&](const Steps& st, int buf) {
-    const size_t s = size_t(st.step());
+  // scales: LDS buffer of the block that a step is in
+  const auto scale_lds = [&](int block) { return 2 * kStageBytes + (block & 1) * kScaleBytes; };
+  // A step's loads in four parts, so that they can be spread over the products of
+  // the step before.
+  const auto issue = [&](const Steps& st, int buf, int block, int part) {
+    const int s = st.s;
     const uint32_t to = lds0 + buf * kStageBytes;
-    const uint32_t act = to + wave * 3 * 1024;
-    if (!DUAL || !st.third()) {
-      const uint8_t* p = pair + s * (4 * kMxPairBytes);
-      dma16(act, p);
-      dma16(act + 1024, p + 16);
-      dma16(act + 2048, p + 32);
-    } else {
-      const uint8_t* p = third + s * (4 * kMxThirdBytes);
-      dma16(act, p);
-      dma16(act + 1024, p + 16);
-    }
-    const uint32_t wt = to + kActBytes + wave * 4 * 1024;
+    if (part == 0) {
+      const uint32_t act = to + wave * 3 * 1024;
+      const uint8_t* p = apair + s * kMxStepPair;
+      dma16(act, pair_off, p);
+      dma16(act + 1024, pair_off, p + kMxChunk);
+      dma16(act + 2048, pair_off, p + 2 * kMxChunk);
+    } else if (part < 3) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) dma16(wt + i * 1024, wsrc[i] + s * 64);
-    dma4(to + kActBytes + kWeightBytes + wave * 256, ascale + s * 4);
-    dma4(to + kActBytes + kWeightBytes + kActScaleBytes + wave * 256, wscale + s * 4);
+      for (int i = 2 * part - 2; i < 2 * part; ++i)
+        dma16(to + kActBytes + (wave * 4 + i) * 1024, w_off,
+              wbase + size_t(tile_row(4 * wave + i)) * (a.cols / 2) + s * 64);
+    } else {
+      if (DUAL && (thirds >> s & 1))
+        dma16(to + kActBytes + kWeightBytes + wave * 1024, third_off, a.third + s * kMxStepThird);
+      const uint32_t sc = lds0 + scale_lds(block);
+      const int at16 = s / kMxScaleSteps * kMxScaleBlock;
+      if (st.fresh()) {
+        if (lane < 16) dma16(sc + wave * 16 * kMxScaleBlock, ascale_off, ascale + at16);
+        if constexpr (BLOCKS)
+          dma16(sc + kActScaleBytes + wave * 64 * kMxScaleBlock, wscale_off, wscale + at16);
+      }
+      if constexpr (!BLOCKS)  // step i of a block: rows' words side by side
+        dma4(sc + kActScaleBytes + (s % kMxScaleSteps) * (kTileCols * 4) + wave * 256, wscale_off,
+             wscale + s * 4);
+    }
   };
 
   const int rh = wave & 1, wq = wave >> 1;  // this wave's half of the rows, quarter of the weights
@@ -375,51 +496,110 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void mx_tile_kernel(const MxArg
   };
   const int tiles_in = min(4, max(0, (m - 64 * rh + 15) / 16));  // row tiles that hold rows
 
-  issue(todo, 0);
+  const int slot = (r * 4 + (q ^ (r >> 2))) * 16;  // where chunk q of a tile's row r lies
+
+  // The loop over the steps, for the row tiles of this wave that hold rows: known
+  // when compiled, so that no branch keeps the reads of one row tile from running
+  // under the products of another (branches cost a fifth).  Every wave passes
+  // the same barriers, whichever form its own half of the rows takes.
+  const auto run = [&](auto row_tiles) {
+  constexpr int NT = decltype(row_tiles)::value;
+#pragma unroll
+  for (int part = 0; part < 4; ++part) issue(todo, 0, 0, part);
   Steps ahead = todo;
-  ahead.next();
+  ++ahead.s;
+  int block = 0, block_ahead = 0;
+  uint32_t sw4[8], sa4[4];  // the lane's scales of a block's steps, this one's lowest
   for (int buf = 0; !todo.done(); buf ^= 1) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();  // this step is in LDS, and the other buffer has been read
-    if (!ahead.done()) {
-      issue(ahead, buf ^ 1);
-      ahead.next();
-    }
+    const bool more = !ahead.done();
+    if (more) block_ahead += ahead.fresh() ? 1 : 0;
+    if constexpr (NT > 0) {
     const uint8_t* from = lds + buf * kStageBytes;
-    const uint8_t* as = from + kActBytes + kWeightBytes;
-    const uint8_t* ws = as + kActScaleBytes;
+    const int si = todo.s % kMxScaleSteps;
+    const uint8_t* ss = lds + scale_lds(block);
+    if (!todo.fresh()) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) sa4[i] >>= 8;
+      if constexpr (BLOCKS)
+#pragma unroll
+        for (int f = 0; f < 8; ++f) sw4[f] >>= 8;
+    } else {
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+        sa4[i] = *reinterpret_cast<const uint32_t*>(ss + (64 * rh + 16 * i + r) * kMxScaleBlock +
+                                                    4 * q);
+      if constexpr (BLOCKS) {
+        // bytes q, 4 + q, 8 + q and 12 + q of the row's 16
+        const uint32_t pick = uint32_t(q) | uint32_t(4 + q) << 8;
+#pragma unroll
+        for (int f = 0; f < 8; ++f) {
+          const uint4 v = *reinterpret_cast<const uint4*>(
+              ss + kActScaleBytes + (16 * weight_tile(f) + r) * kMxScaleBlock);
+          sw4[f] = __builtin_amdgcn_perm(v.y, v.x, pick) & 0xffffu |
+                   __builtin_amdgcn_perm(v.w, v.z, pick) << 16;
+        }
+      }
+    }
     uint4 w[8];
-    int sw[8];
 #pragma unroll
     for (int f = 0; f < 8; ++f) {
       const int wt = weight_tile(f);
-      w[f] = *reinterpret_cast<const uint4*>(from + kActBytes + wt * 1024 + lane * 16);
-      sw[f] = ws[(wt >> 2) * 256 + ((wt & 3) * 16 + r) * 4 + q];
+      w[f] = *reinterpret_cast<const uint4*>(from + kActBytes + wt * 1024 + slot);
+      if constexpr (!BLOCKS)
+        sw4[f] = ss[kActScaleBytes + si * (kTileCols * 4) + (16 * wt + r) * 4 + q];
     }
-    const bool third_step = DUAL && todo.third();
+    uint4 c[2][3];
+    const auto read = [&](int i) {
+      const uint8_t* src = from + (4 * rh + i) * 3 * 1024 + slot;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (i >= tiles_in) break;
-      const int rt = 4 * rh + i;
-      const uint8_t* src = from + rt * 3 * 1024 + lane * 16;
-      const int sa = as[rt * 256 + r * 4 + q];
-      const uint4 c0 = *reinterpret_cast<const uint4*>(src);
-      const uint4 c1 = *reinterpret_cast<const uint4*>(src + 1024);
-      const uint32_t b0[6] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y};
-      if (third_step) {
+      for (int j = 0; j < 3; ++j) c[i & 1][j] = *reinterpret_cast<const uint4*>(src + j * 1024);
+    };
+    read(0);
 #pragma unroll
-        for (int f = 0; f < 8; ++f) mx_mma(acc[f][i], w[f], sw[f], b0, sa - 2 * kMxTokenShift);
-      } else {
-        const uint4 c2 = *reinterpret_cast<const uint4*>(src + 2048);
-        const uint32_t b1[6] = {c1.z, c1.w, c2.x, c2.y, c2.z, c2.w};
+    for (int i = 0; i < NT; ++i) {
+      // the next row tile's reads and a part of the next step's loads go out
+      // before this row tile's products
+      if (i + 1 < NT) read(i + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      if (more) issue(ahead, buf ^ 1, block_ahead, i);
+      const uint4(&d)[3] = c[i & 1];
+      const int sa = int(sa4[i]);
+      const uint32_t b0[6] = {d[0].x, d[0].y, d[0].z, d[0].w, d[1].x, d[1].y};
+      const uint32_t b1[6] = {d[1].z, d[1].w, d[2].x, d[2].y, d[2].z, d[2].w};
 #pragma unroll
-        for (int f = 0; f < 8; ++f) mx_mma(acc[f][i], w[f], sw[f], b0, sa);
+      for (int f = 0; f < 8; ++f) mx_mma(acc[f][i], w[f], int(sw4[f]), b0, sa);
 #pragma unroll
-        for (int f = 0; f < 8; ++f)
-          mx_mma(acc[f][i], w[f], sw[f], b1, sa - (DUAL ? kMxTokenShift : kMxInterShift));
+      for (int f = 0; f < 8; ++f)
+        mx_mma(acc[f][i], w[f], int(sw4[f]), b1, sa - (DUAL ? kMxTokenShift : kMxInterShift));
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (DUAL && (thirds >> todo.s & 1)) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const uint4 d = *reinterpret_cast<const uint4*>(from + kActBytes + kWeightBytes +
+                                                        (4 * rh + i) * 1024 + slot);
+#pragma unroll
+        for (int f = 0; f < 8; ++f) mx_mma_third(acc[f][i], w[f], int(sw4[f]), d, int(sa4[i]));
       }
     }
-    todo.next();
+    }
+    if (more) {
+#pragma unroll
+      for (int part = NT; part < 4; ++part) issue(ahead, buf ^ 1, block_ahead, part);
+      ++ahead.s;
+    }
+    ++todo.s;
+    block += todo.fresh() ? 1 : 0;
+  }
+  };
+  switch (tiles_in) {
+    case 0: run(std::integral_constant<int, 0>{}); break;
+    case 1: run(std::integral_constant<int, 1>{}); break;
+    case 2: run(std::integral_constant<int, 2>{}); break;
+    case 3: run(std::integral_constant<int, 3>{}); break;
+    default: run(std::integral_constant<int, 4>{}); break;
   }
 
   if constexpr (DUAL) {
@@ -428,7 +608,6 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void mx_tile_kernel(const MxArg
     float* hs = reinterpret_cast<float*>(lds) + wave * 32 * kPitch;
     static_assert(kTileWaves * 32 * kPitch * 4 <= kTileLds, "h staging");
     const int f0 = fb * kCols + 64 * wq;
-    const int hgroups = a.features / kMxGroup;
     __syncthreads();
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -453,39 +632,78 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void mx_tile_kernel(const MxArg
           v[4 * c] = x.x, v[4 * c + 1] = x.y, v[4 * c + 2] = x.z, v[4 * c + 3] = x.w;
         }
         int s;
-        u32x6 h0, h1, h2;
-        mx_split<false>(v, s, h0, h1, h2);
-        const size_t to = size_t(p0 + row) * hgroups + f / kMxGroup;
-        mx_store_pair(a.hpair + to * kMxPairBytes, h0, h1);
-        a.hscale[to] = uint8_t(s);
+        u32x6 h0, h1;
+        uint4 none;
+        mx_split<false>(v, s, h0, h1, none);
+        const size_t to = size_t(p0 + row) * mx_steps(a.features);
+        mx_store_pair(a.hpair + to * kMxStepPair, f / kMxGroup, h0, h1);
+        a.hscale[size_t(p0 + row) * mx_scale_row(a.features) + mx_scale_at(f / kMxGroup)] =
+            uint8_t(s);
       }
       __syncthreads();
     }
   } else {
+    // 16 rows x 128 features at a time through the wave's own LDS, so that 16
+    // lanes store one row's 256 bytes (8-byte stores from the accumulators took a
+    // third of the kernel's time)
+    constexpr int kPitch = 272;
+    uint8_t* ys = lds + wave * 16 * kPitch;
+    const int f0 = fb * kCols + 128 * wq;
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int row = 64 * rh + 16 * i + r;
-      if (row >= m) continue;
-      uint16_t* y = a.y + size_t(a.order[p0 + row]) * a.features;
+      const int row0 = 64 * rh + 16 * i;
+      if (row0 >= m || f0 >= a.features) break;
+      const size_t own = row0 + r < m ? a.order[p0 + row0 + r] : 0;
+      uint16_t o[32];
+      if constexpr (HALF) {
 #pragma unroll
-      for (int f = 0; f < 8; ++f) {
-        const int c = fb * kCols + 128 * wq + 16 * f + 4 * q;
-        if (c >= a.features) continue;
-        const f32x4 v = acc[f][i];
-        *reinterpret_cast<uint2*>(y + c) = make_uint2(uint32_t(f2bf(v[0])) | uint32_t(f2bf(v[1])) << 16,
-                                                      uint32_t(f2bf(v[2])) | uint32_t(f2bf(v[3])) << 16);
+        for (int g = 0; g < 4; ++g) {  // 32 features: two tiles over the row's four lanes
+          uint32_t top = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            top = max(top, __float_as_uint(acc[2 * g + j / 4][i][j & 3]) & 0x7fffffffu);
+          top = max(top, uint32_t(__float_as_int(xor_lane<16>(__int_as_float(int(top))))));
+          top = max(top, uint32_t(__float_as_int(xor_lane<32>(__int_as_float(int(top))))));
+          const int sc = half_scale(top);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) o[8 * g + j] = half_of(acc[2 * g + j / 4][i][j & 3], sc);
+          if (q == g && row0 + r < m && f0 + 32 * g < a.features)
+            a.yscale[(own * a.features + f0) / kMxGroup + g] = uint8_t(sc);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) o[j] = f2bf(acc[j / 4][i][j & 3]);
       }
+#pragma unroll
+      for (int f = 0; f < 8; ++f)
+        *reinterpret_cast<uint2*>(ys + r * kPitch + (16 * f + 4 * q) * 2) =
+            make_uint2(uint32_t(o[4 * f]) | uint32_t(o[4 * f + 1]) << 16,
+                       uint32_t(o[4 * f + 2]) | uint32_t(o[4 * f + 3]) << 16);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int row = 4 * j + (lane >> 4), c = f0 + 8 * (lane & 15);
+        const uint4 v = *reinterpret_cast<const uint4*>(ys + row * kPitch + (lane & 15) * 16);
+        if (row0 + row < m && c < a.features)
+          *reinterpret_cast<uint4*>(a.y + size_t(a.order[p0 + row0 + row]) * a.features + c) = v;
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
   }
 }
 
-template <bool DUAL>
+template <bool DUAL, bool HALF>
 int launch_tile(const MxArgs& a, int max_tiles, hipStream_t st) {
   constexpr int kCols = DUAL ? kTileCols / 2 : kTileCols;
   const int64_t blocks = (int64_t(max_tiles) * ((a.features + kCols - 1) / kCols) + 7) / 8 * 8;
   PMOE_REQUIRE(blocks < (int64_t(1) << 31), "experts: too many tiles for one call");
   ProfScope prof_scope(DUAL ? K_MX_GATEUP : K_MX_DOWN, st);
-  mx_tile_kernel<DUAL><<<unsigned(blocks), 64 * kTileWaves, 0, st>>>(a);
+  const int64_t scales = DUAL ? a.s0 | a.s1 : a.s0;
+  if (a.cols % kStep == 0 && (scales | a.expert_bytes) % 16 == 0)
+    mx_tile_kernel<DUAL, true, HALF><<<unsigned(blocks), 64 * kTileWaves, 0, st>>>(a);
+  else
+    mx_tile_kernel<DUAL, false, HALF><<<unsigned(blocks), 64 * kTileWaves, 0, st>>>(a);
   PMOE_LAUNCH_CHECK("mx_tile_kernel");
   return PMOE_OK;
 }
@@ -498,6 +716,8 @@ int mx_tile_rows(const pmoe_geom* g, int n, int kk, int n_experts) {
   if (g->hidden % 128 || g->inter % 128 ||
       (g->off[PMOE_GATE_S] | g->off[PMOE_UP_S] | g->off[PMOE_DOWN_S]) % 4)
     return kSmallRows;
+  // the tokens' pieces within the large tiles' 32-bit offsets
+  if (int64_t(n) * mx_steps(g->hidden) * kMxStepPair >= int64_t(1) << 32) return kSmallRows;
   if (v && v[0] == '0') return kSmallRows;
   if (v && v[0] == '1') return kTileRows;
   return int64_t(n) * kk >= 16L * n_experts ? kTileRows : kSmallRows;
@@ -508,8 +728,9 @@ int mx_experts(const MxPlan& p, hipStream_t st) {
   const pmoe_geom* g = p.geom;
   {
     ProfScope prof_scope(K_MX_SPLIT, st);
-    mx_split_kernel<<<p.n, 256, 0, st>>>(p.x, p.n, g->hidden / kMxGroup, p.xpair, p.xthird,
-                                         p.xscale, p.xsteps);
+    mx_split_kernel<<<p.n, 256, 0, st>>>(p.x, p.n, g->hidden / kMxGroup, mx_steps(g->hidden),
+                                         mx_scale_row(g->hidden), p.xpair, p.xthird, p.xscale,
+                                         p.xsteps);
     PMOE_LAUNCH_CHECK("mx_split_kernel");
   }
   const bool large = p.tile_rows == kTileRows;
@@ -526,15 +747,32 @@ int mx_experts(const MxPlan& p, hipStream_t st) {
   a.cols = g->hidden;
   a.pair = p.xpair, a.third = p.xthird, a.ascale = p.xscale, a.asteps = p.xsteps;
   a.hpair = p.hpair, a.hscale = p.hscale;
-  if (int rc = large ? launch_tile<true>(a, p.max_tiles, st)
-                     : launch_small<true>(a, p.max_tiles, st))
+  if (int rc = large ? launch_tile<true, false>(a, p.max_tiles, st)
+                     : launch_small<true, false>(a, p.max_tiles, st))
     return rc;
   a.w0 = g->off[PMOE_DOWN_W], a.s0 = g->off[PMOE_DOWN_S];
   a.features = g->hidden;
   a.cols = g->inter;
   a.pair = p.hpair, a.third = nullptr, a.ascale = p.hscale, a.asteps = nullptr;
   a.y = p.y;
-  return large ? launch_tile<false>(a, p.max_tiles, st) : launch_small<false>(a, p.max_tiles, st);
+  a.yscale = p.yscale;
+  if (p.yscale)
+    return large ? launch_tile<false, true>(a, p.max_tiles, st)
+                 : launch_small<false, true>(a, p.max_tiles, st);
+  return large ? launch_tile<false, false>(a, p.max_tiles, st)
+               : launch_small<false, false>(a, p.max_tiles, st);
+}
+
+int mx_combine(const uint16_t* y, const uint8_t* yscale, const float* w, const int32_t* inv,
+               const float* shared_logit, int n, int k, int kk, int d, uint16_t* out,
+               hipStream_t st) {
+  const int blocks_row = (d / 8 + 255) / 256;
+  PMOE_REQUIRE(int64_t(n) * blocks_row < (int64_t(1) << 31), "experts: too many rows for one call");
+  ProfScope prof_scope(K_COMBINE, st);
+  mx_combine_kernel<<<unsigned(n) * blocks_row, 256, 0, st>>>(y, yscale, w, inv, shared_logit, k,
+                                                             kk, d, blocks_row, out);
+  PMOE_LAUNCH_CHECK("mx_combine_kernel");
+  return PMOE_OK;
 }
 
 }  // namespace pmoe

@@ -4,19 +4,19 @@
 // A group of 32 values gets a power of two 2^e that brings its largest
 // magnitude into [4, 8), and each value a is written as
 //
-//   a = 2^e (p0 + p1 / 16 + p2 / 256) + rest     (tokens)
+//   a = 2^e (p0 + p1 / 16 + p2 / 1024) + rest    (tokens)
 //   a = 2^e (p0 + p1 / 32) + rest                (intermediates)
 //
-// with pieces of 1 sign, 2 exponent and 3 mantissa bits (E2M3: steps of 1/8 up
-// to 2, 1/4 up to 4, 1/2 up to 7.5), each the nearest to what the ones before
-// leave over.
+// with p0 and p1 of 1 sign, 2 exponent and 3 mantissa bits (E2M3: steps of 1/8 up
+// to 2, 1/4 up to 4, 1/2 up to 7.5) and p2 of 1 mantissa bit (E2M1, the weights'
+// format), each the nearest to what the ones before leave over.
 //
 // Tokens are bf16.  Two pieces hold a value of at least an eighth of the
 // group's largest exactly and any other to 2^-8 2^e, i.e. to 2^-10 of the
-// largest.  The third is kept only where one value stands out of its group
+// largest, the rest of a value being at most 4 / 1024 2^e.  p2 is kept only where one value stands out of its group
 // (its square is more than the sum of the other 31's, in trained models the few
 // channels with huge activations), so that the others are not rounded to a
-// step that it sets: they are then off by at most 2^-14 of the largest.
+// step that it sets: they are then off by at most 2^-10 2^e, 2^-12 of the largest.
 //
 // Intermediates are fp32.  The second piece's smaller unit makes its steps half
 // as wide where most values are (2^-9 2^e below 2, 2^-8 2^e below 4, 2^-7 2^e above,
@@ -38,13 +38,27 @@ typedef float f32x32 __attribute__((ext_vector_type(32)));
 typedef uint32_t u32x6 __attribute__((ext_vector_type(6)));
 
 constexpr int kMxGroup = 32;
-constexpr int kMxPieceBytes = 24;     // 32 values of 6 bits
-constexpr int kMxPairBytes = 48;      // p0, p1 of a group
-constexpr int kMxThirdBytes = 32;     // p2 of a group, padded to whole 16 bytes
+// A row of pieces goes by steps of 128 values (4 groups, the last step padded):
+// p0 and p1 of a group are 48 bytes, chunk i of the step's groups side by side
+// in 64 bytes, so that lanes side by side fetch whole 64-byte stretches.
+constexpr int kMxStepGroups = 4;
+constexpr int kMxStepPair = 192;      // 3 chunks of 4 x 16 bytes
+constexpr int kMxStepThird = 64;      // p2: 4 x 16 bytes
+constexpr int kMxChunk = 64;
+// Their scales go by 512 values, 16 bytes: byte 4 q + i is group 4 i + q's, so
+// that a lane finds its group's scales of four steps in one word.
+constexpr int kMxScaleSteps = 4;
+constexpr int kMxScaleBlock = 16;
+
+__host__ __device__ constexpr int mx_steps(int cols) {
+  return (cols / kMxGroup + kMxStepGroups - 1) / kMxStepGroups;
+}
+
 constexpr int kMxTokenShift = 4;      // p1's power of two below p0's
+constexpr int kMxThirdShift = 10;     // p2's
 constexpr int kMxInterShift = 5;
-// The least scale byte of p0: the last piece's, 8 or 5 below, is at least 1.
-constexpr int kMxMinToken = 9, kMxMinInter = 6;
+// The least scale byte of p0: the last piece's is at least 1.
+constexpr int kMxMinToken = kMxThirdShift + 1, kMxMinInter = kMxInterShift + 1;
 
 // 32 floats over 2^x to E2M3, nearest even.  The instruction takes the even
 // and the odd values apart, and writes its result while it still reads its
@@ -73,7 +87,7 @@ __device__ __forceinline__ float mx_pow2(int biased) {
 // token's, with p2 (zeros where no value stands out, and then false).
 template <bool THIRD>
 __device__ __forceinline__ bool mx_split(float (&v)[32], int& scale, u32x6& p0, u32x6& p1,
-                                         u32x6& p2) {
+                                         uint4& p2) {
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
@@ -101,30 +115,47 @@ __device__ __forceinline__ bool mx_split(float (&v)[32], int& scale, u32x6& p0, 
   for (int i = 0; i < 32; ++i) v[i] -= b[i];
   const float f1 = mx_pow2(s - (THIRD ? kMxTokenShift : kMxInterShift));
   p1 = mx_to_fp6(v, f1);
-  p2 = u32x6{0, 0, 0, 0, 0, 0};
+  p2 = make_uint4(0, 0, 0, 0);
   if constexpr (THIRD) {
     if (peak) {
       b = mx_from_fp6(p1, f1);
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] -= b[i];
-      p2 = mx_to_fp6(v, mx_pow2(s - 2 * kMxTokenShift));
+      const float f2 = mx_pow2(s - kMxThirdShift);
+      uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[i], v[8 * i], v[8 * i + 1], f2, 0);
+        w[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[i], v[8 * i + 2], v[8 * i + 3], f2, 1);
+        w[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[i], v[8 * i + 4], v[8 * i + 5], f2, 2);
+        w[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[i], v[8 * i + 6], v[8 * i + 7], f2, 3);
+      }
+      p2 = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
   scale = e == 255 ? 255 : s;
   return peak;
 }
 
-__device__ __forceinline__ void mx_store_pair(uint8_t* dst, u32x6 p0, u32x6 p1) {
-  uint4* d = reinterpret_cast<uint4*>(dst);
-  d[0] = make_uint4(p0[0], p0[1], p0[2], p0[3]);
-  d[1] = make_uint4(p0[4], p0[5], p1[0], p1[1]);
-  d[2] = make_uint4(p1[2], p1[3], p1[4], p1[5]);
+__host__ __device__ constexpr int mx_scale_row(int cols) {
+  return (mx_steps(cols) + kMxScaleSteps - 1) / kMxScaleSteps * kMxScaleBlock;
 }
 
-__device__ __forceinline__ void mx_store_third(uint8_t* dst, u32x6 p2) {
-  uint4* d = reinterpret_cast<uint4*>(dst);
-  d[0] = make_uint4(p2[0], p2[1], p2[2], p2[3]);
-  d[1] = make_uint4(p2[4], p2[5], 0, 0);
+// Where group g's scale lies in a row of scales.
+__device__ __forceinline__ int mx_scale_at(int g) {
+  return (g & ~15) + 4 * (g & 3) + (g >> 2 & 3);
+}
+
+// Group g's pieces into a row of pieces.
+__device__ __forceinline__ void mx_store_pair(uint8_t* row, int g, u32x6 p0, u32x6 p1) {
+  uint8_t* d = row + (g >> 2) * kMxStepPair + (g & 3) * 16;
+  *reinterpret_cast<uint4*>(d) = make_uint4(p0[0], p0[1], p0[2], p0[3]);
+  *reinterpret_cast<uint4*>(d + kMxChunk) = make_uint4(p0[4], p0[5], p1[0], p1[1]);
+  *reinterpret_cast<uint4*>(d + 2 * kMxChunk) = make_uint4(p1[2], p1[3], p1[4], p1[5]);
+}
+
+__device__ __forceinline__ void mx_store_third(uint8_t* row, int g, uint4 p2) {
+  *reinterpret_cast<uint4*>(row + (g >> 2) * kMxStepThird + (g & 3) * 16) = p2;
 }
 
 }  // namespace pmoe
