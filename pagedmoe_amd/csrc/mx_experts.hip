@@ -13,6 +13,7 @@
 #include <hip/hip_fp16.h>
 #include <stdlib.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "mx_experts.h"
@@ -162,6 +163,33 @@ __global__ __launch_bounds__(256) void mx_split_kernel(const uint16_t* __restric
   }
 }
 
+// ---------------------------------------------------------------- memory to LDS
+
+// 16 bytes (4 bytes) a lane from base + voff to LDS [lds, lds + 1024) ([.., +
+// 256)), lane l at 16 l (4 l).  base and lds are the wave's.
+__device__ __forceinline__ void dma16(uint32_t lds, uint32_t voff, const uint8_t* base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(uniform_ptr(base))
+               : "memory");
+}
+
+__device__ __forceinline__ void dma4(uint32_t lds, uint32_t voff, const uint8_t* base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(uniform_ptr(base))
+               : "memory");
+}
+
+// Rows of 4, 8 or 16 chunks of 16 bytes lie in LDS with chunk p of row r at place
+// p ^ swizzle(r).  A 16-byte LDS read takes its lanes in sets of 16: 0-3, 12-15,
+// 20-23, 24-27 and so on, which here are rows 0-3 and 12-15 of one chunk and 4-11
+// of the next (lane 16 q + r reads chunk 4 i + q of row r); with these the 16
+// meet the 16 groups of four banks once each.
+__device__ __forceinline__ int swizzle4(int r) { return -(r >> 2) & 3; }
+__device__ __forceinline__ int swizzle8(int r) { return (r >> 1 & 4) | (r & 2); }
+__device__ __forceinline__ int swizzle16(int r) { return (r & 3) << 1 | (r & 8); }
+
 // ---------------------------------------------------------------- small tiles
 
 constexpr int kSmallRows = 16;   // activation rows a tile
@@ -170,10 +198,10 @@ constexpr int kStep = 512;       // reduction that a wave takes at a time
 constexpr int kMaxWaves = 8;
 
 // One tile of at most 16 rows of an expert times 32 features (DUAL: 32 gate
-// and the same 32 up features).  The waves share the reduction: wave w takes
-// steps w, w + waves, ... of 512, all loads of a step in flight at once, and
-// the partial sums meet in LDS.  FULL: the reduction is whole steps.
-template <bool DUAL, bool FULL, bool HALF>
+// and the same 32 up features), for reductions of any number of groups.  The
+// waves share the reduction: wave w takes steps w, w + waves, ... of 512, and
+// the partial sums meet in LDS.
+template <bool DUAL, bool HALF>
 __global__ __launch_bounds__(64 * kMaxWaves) void mx_small_kernel(const MxArgs a) {
   constexpr int NF = DUAL ? 4 : 2;  // 16-feature tiles: gate, gate, up, up
   __shared__ float s_red[kMaxWaves][NF * 4][64];
@@ -225,7 +253,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void mx_small_kernel(const MxArgs a
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int g = 16 * j + 4 * i + q;
-      const bool in = FULL || g < groups;
+      const bool in = g < groups;
 #pragma unroll
       for (int f = 0; f < NF; ++f) {
         w[f][i] = in ? *reinterpret_cast<const uint4*>(wrow[f] + size_t(g) * 16)
@@ -236,7 +264,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void mx_small_kernel(const MxArgs a
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int g = 16 * j + 4 * i + q;
-      const bool in = FULL || g < groups;
+      const bool in = g < groups;
       const int gc = in ? g : 0;
       const uint4* src =
           reinterpret_cast<const uint4*>(pair + (gc >> 2) * kMxStepPair + (gc & 3) * 16);
@@ -311,11 +339,205 @@ int launch_small(const MxArgs& a, int max_tiles, hipStream_t st) {
   const int64_t blocks = int64_t(max_tiles) * (a.features / kSmallCols);
   PMOE_REQUIRE(blocks < (int64_t(1) << 31) / 1, "experts: too many tiles for one call");
   ProfScope prof_scope(DUAL ? K_MX_GATEUP : K_MX_DOWN, st);
-  if (a.cols % kStep == 0)
-    mx_small_kernel<DUAL, true, HALF><<<unsigned(blocks), 64 * waves, 0, st>>>(a);
-  else
-    mx_small_kernel<DUAL, false, HALF><<<unsigned(blocks), 64 * waves, 0, st>>>(a);
+  mx_small_kernel<DUAL, HALF><<<unsigned(blocks), 64 * waves, 0, st>>>(a);
   PMOE_LAUNCH_CHECK("mx_small_kernel");
+  return PMOE_OK;
+}
+
+// ---------------------------------------------------------------- streamed tiles
+
+constexpr int kStreamStep = 256;                   // reduction that a wave takes at a time
+constexpr int kStreamRows = 64;                    // weight rows a block
+constexpr int kStreamWave = kStreamRows * 128 + 2 * kStreamRows * 4;  // LDS of a wave
+
+// As mx_small_kernel, for reductions of whole steps of 128: one tile of at most
+// 16 rows times 64 weight rows (DUAL: 32 gate and the same 32 up features; 64
+// features otherwise).  Bound by the weights' stream: a wave's 64 rows x 128
+// bytes go straight into its own LDS, 8 lanes side by side on a row's 128 bytes,
+// so that nothing waits for registers and the fetches are whole lines; two
+// blocks a CU keep 136 KB in flight.  (Loads into registers in the products' own
+// lane order, 16 bytes of 64 different rows an instruction, reached 3 TB/s.)
+template <bool DUAL, bool HALF>
+__global__ __launch_bounds__(64 * kMaxWaves, 4) void mx_stream_kernel(const MxArgs a) {
+  constexpr int NF = 4;
+  constexpr int kCols = DUAL ? kStreamRows / 2 : kStreamRows;  // features a block
+  extern __shared__ __attribute__((aligned(1024))) uint8_t dyn[];
+  const int fblocks = (a.features + kCols - 1) / kCols;
+  const int t = blockIdx.x / fblocks;
+  const int fb = blockIdx.x - t * fblocks;
+  if (t >= *a.n_tiles) return;
+  const int4 tile = a.tiles[t];  // {slot, first row, rows of the expert, offset}
+  const int m = min(kSmallRows, tile.z - tile.y);
+  const int p0 = tile.w + tile.y;
+  const int waves = blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int cols_in = min(kCols, a.features - fb * kCols);
+  if (tile.x < 0) {  // not resident: exact zero rows
+    if constexpr (!DUAL) {
+      for (int i = threadIdx.x; i < m * kCols; i += blockDim.x) {
+        const int c = i % kCols;
+        if (c >= cols_in) continue;
+        const size_t at = size_t(a.order[p0 + i / kCols]) * a.features + fb * kCols + c;
+        a.y[at] = 0;
+        if (HALF && c % kMxGroup == 0) a.yscale[at / kMxGroup] = 1;
+      }
+    }
+    return;
+  }
+  const int r = lane & 15, q = lane >> 4;
+  const int groups = a.cols / kMxGroup, steps = groups / kMxStepGroups;
+  const uint8_t* base = a.slab + size_t(tile.x) * size_t(a.expert_bytes);
+  const uint32_t row_bytes = a.cols / 2;
+  // weight tile f: 16 features from f16 of projection f / 2 (DUAL); tiles past the
+  // projection load its last one and are not used
+  const auto feature0 = [&](int f) {
+    return min(fb * kCols + 16 * (DUAL ? f & 1 : f), a.features - 16);
+  };
+  const uint8_t* wbase[NF];
+#pragma unroll
+  for (int f = 0; f < NF; ++f)
+    wbase[f] = base + (DUAL && f > 1 ? a.w1 : a.w0) + size_t(feature0(f)) * row_bytes;
+  // rows 8 i + lane / 8 of a tile; their chunks' order goes by the row
+  const int lrow = lane >> 3;
+  const int lp[2] = {(lane & 7) ^ swizzle8(lrow), (lane & 7) ^ swizzle8(lrow + 8)};
+  const uint8_t* sbase = base + (DUAL && q > 1 ? a.s1 : a.s0) + size_t(feature0(q) + r) * groups;
+  uint8_t* own = dyn + wave * kStreamWave;
+  const uint32_t own_lds = __builtin_amdgcn_readfirstlane(
+      uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)own)));
+  const bool live = r < m;
+  const size_t arow = live ? (DUAL ? size_t(a.order[p0 + r] / a.kk) : size_t(p0 + r)) : 0;
+  const uint8_t* pair = a.pair + arow * steps * kMxStepPair + q * 16;
+  const uint8_t* third = DUAL ? a.third + arow * steps * kMxStepThird + q * 16 : nullptr;
+  const uint8_t* ascale = a.ascale + arow * mx_scale_row(a.cols) + q * 4;
+
+  f32x4 acc[NF];
+#pragma unroll
+  for (int f = 0; f < NF; ++f) acc[f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int j = wave; 2 * j < steps; j += waves) {
+    const bool two = 2 * j + 1 < steps;  // the step's second half is there
+    // this step's activations (rows that are not there: zeros)
+    uint4 c[2][3], d[2];
+    uint32_t sa4 = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int k = 0; k < 3; ++k) c[i][k] = make_uint4(0, 0, 0, 0);
+      d[i] = make_uint4(0, 0, 0, 0);
+    }
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (i == 0 || two) {
+          const uint8_t* src = pair + (2 * j + i) * kMxStepPair;
+#pragma unroll
+          for (int k = 0; k < 3; ++k) c[i][k] = *reinterpret_cast<const uint4*>(src + k * kMxChunk);
+          if constexpr (DUAL)
+            d[i] = *reinterpret_cast<const uint4*>(third + (2 * j + i) * kMxStepThird);
+        }
+      }
+      sa4 = *reinterpret_cast<const uint32_t*>(ascale + (j >> 1) * kMxScaleBlock);
+    }
+    // the LDS reads of the step before are done
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (two || lp[i] < 4)
+          dma16(own_lds + f * 2048 + i * 1024, lrow * row_bytes + lp[i] * 16,
+                wbase[f] + size_t(8 * i) * row_bytes + j * 128);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (i == 0 || two)
+        dma4(own_lds + NF * 2048 + i * 256, uint32_t(sbase - base) + (2 * j + i) * 4, base);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (i && !two) break;
+      const int at = (r * 8 + ((4 * i + q) ^ swizzle8(r))) * 16;
+      const int sa = int(sa4 >> (8 * (2 * (j & 1) + i)));
+      uint4 w[NF];
+      int sw[NF];
+#pragma unroll
+      for (int f = 0; f < NF; ++f) {
+        w[f] = *reinterpret_cast<const uint4*>(own + f * 2048 + at);
+        sw[f] = own[NF * 2048 + i * 256 + (16 * f + r) * 4 + q];
+      }
+      const uint32_t b0[6] = {c[i][0].x, c[i][0].y, c[i][0].z, c[i][0].w, c[i][1].x, c[i][1].y};
+      const uint32_t b1[6] = {c[i][1].z, c[i][1].w, c[i][2].x, c[i][2].y, c[i][2].z, c[i][2].w};
+#pragma unroll
+      for (int f = 0; f < NF; ++f) mx_mma(acc[f], w[f], sw[f], b0, sa);
+#pragma unroll
+      for (int f = 0; f < NF; ++f)
+        mx_mma(acc[f], w[f], sw[f], b1, sa - (DUAL ? kMxTokenShift : kMxInterShift));
+      if constexpr (DUAL)
+#pragma unroll
+        for (int f = 0; f < NF; ++f) mx_mma_third(acc[f], w[f], sw[f], d[i], sa);
+    }
+  }
+  // partial sums meet in LDS: [wave][4 f + i][lane]
+  float(*red)[16][64] = reinterpret_cast<float(*)[16][64]>(dyn);
+  float(*hs)[kCols + 1] = reinterpret_cast<float(*)[kCols + 1]>(dyn + waves * sizeof(red[0]));
+  __syncthreads();
+#pragma unroll
+  for (int f = 0; f < NF; ++f)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) red[wave][4 * f + i][lane] = acc[f][i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < kSmallRows * kCols; i += blockDim.x) {
+    const int row = i / kCols, c = i % kCols;
+    if (row >= m) break;  // whole halves of a wave
+    const int src = (c & 15) / 4 * 16 + row;
+    float v = 0.0f, u = 0.0f;
+    for (int k = 0; k < waves; ++k) {
+      v += red[k][4 * (c >> 4) + (c & 3)][src];
+      if constexpr (DUAL) u += red[k][4 * (2 + (c >> 4)) + (c & 3)][src];
+    }
+    if constexpr (DUAL) {
+      hs[row][c] = silu_fast(v) * u;
+    } else if (c < cols_in) {  // (a multiple of 32)
+      const size_t at = size_t(a.order[p0 + row]) * a.features + fb * kCols + c;
+      if constexpr (HALF) {
+        const int sc = half_scale(half_wave_max(__float_as_uint(v) & 0x7fffffffu));
+        a.y[at] = half_of(v, sc);
+        if (c % kMxGroup == 0) a.yscale[at / kMxGroup] = uint8_t(sc);
+      } else {
+        a.y[at] = f2bf(v);
+      }
+    }
+  }
+  if constexpr (DUAL) {
+    __syncthreads();
+    if (int(threadIdx.x) < m) {
+      float v[32];
+#pragma unroll
+      for (int c = 0; c < 32; ++c) v[c] = hs[threadIdx.x][c];
+      int s;
+      u32x6 h0, h1;
+      uint4 none;
+      mx_split<false>(v, s, h0, h1, none);
+      const size_t row = p0 + threadIdx.x;
+      mx_store_pair(a.hpair + row * mx_steps(a.features) * kMxStepPair, fb, h0, h1);
+      a.hscale[row * mx_scale_row(a.features) + mx_scale_at(fb)] = uint8_t(s);
+    }
+  }
+}
+
+template <bool DUAL, bool HALF>
+int launch_stream(const MxArgs& a, int max_tiles, hipStream_t st) {
+  constexpr int kCols = DUAL ? kStreamRows / 2 : kStreamRows;
+  const int steps = (a.cols + kStreamStep - 1) / kStreamStep;
+  const int rounds = (steps + kMaxWaves - 1) / kMaxWaves;
+  const int waves = (steps + rounds - 1) / rounds;
+  const int64_t blocks = int64_t(max_tiles) * ((a.features + kCols - 1) / kCols);
+  PMOE_REQUIRE(blocks < (int64_t(1) << 31), "experts: too many tiles for one call");
+  const size_t lds = std::max<size_t>(size_t(waves) * kStreamWave,
+                                      size_t(waves) * 4096 + kSmallRows * (kCols + 1) * 4);
+  ProfScope prof_scope(DUAL ? K_MX_GATEUP : K_MX_DOWN, st);
+  mx_stream_kernel<DUAL, HALF><<<unsigned(blocks), 64 * waves, lds, st>>>(a);
+  PMOE_LAUNCH_CHECK("mx_stream_kernel");
   return PMOE_OK;
 }
 
@@ -333,22 +555,6 @@ constexpr int kActScaleBytes = kTileRows * kMxScaleBlock;
 constexpr int kScaleBytes = kActScaleBytes + kTileCols * kMxScaleBlock;
 constexpr int kTileLds = 2 * (kStageBytes + kScaleBytes);
 
-// 16 bytes (4 bytes) a lane from base + voff to LDS [lds, lds + 1024) ([.., +
-// 256)), lane l at 16 l (4 l).  base and lds are the wave's.
-__device__ __forceinline__ void dma16(uint32_t lds, uint32_t voff, const uint8_t* base) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-               :
-               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(uniform_ptr(base))
-               : "memory");
-}
-
-__device__ __forceinline__ void dma4(uint32_t lds, uint32_t voff, const uint8_t* base) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
-               :
-               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(uniform_ptr(base))
-               : "memory");
-}
-
 // The steps of a tile's reduction: s done of n.
 struct Steps {
   int s, n;
@@ -360,11 +566,10 @@ struct Steps {
 // One tile of at most 128 rows of an expert times 512 weight rows (DUAL: 256
 // gate and the same 256 up features).  Each wave holds 64 rows times 128 weight
 // rows in its accumulators.  A step of 128 goes from memory straight into LDS,
-// 16 rows of 64 bytes an instruction: lane l fetches chunk (l & 3) ^ (l >> 4) of
-// row l >> 2, so that four lanes side by side fetch one 64-byte stretch (lanes
-// in the products' own order, 16 rows side by side, cost the cache four times
-// the accesses and bound the kernel) and the 16 lanes that read one chunk of 16
-// rows back meet 16 different banks of 16 bytes.  The next step's loads are in
+// 16 rows of 64 bytes an instruction: four lanes side by side fetch one 64-byte
+// stretch (lanes in the products' own order, 16 rows side by side, cost the
+// cache four times the accesses and bound the kernel), in an order that keeps the
+// reads back free of bank conflicts (swizzle4).  The next step's loads are in
 // flight while this one's products run.
 // Scales come 16 bytes a row, those of four steps.  BLOCKS: the reduction is
 // whole stretches of 512, so that the weights' lie on 16 bytes too; otherwise
@@ -409,7 +614,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void mx_tile_kernel(const MxArg
   // weight tiles 4 wave .. + 3, now and then their scales.  Offsets from the
   // wave's own bases; a tile's intermediate rows follow each other, tokens lie
   // anywhere in less than 4 GiB (mx_tile_rows).
-  const int lr = lane >> 2, lq = (lane & 3) ^ (lane >> 4);
+  const int lr = lane >> 2, lq = (lane & 3) ^ swizzle4(lr);
   const int steps = groups / kMxStepGroups;
   const auto act_row = [&](int row) {
     const int k = row < m ? row : 0;
@@ -496,7 +701,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void mx_tile_kernel(const MxArg
   };
   const int tiles_in = min(4, max(0, (m - 64 * rh + 15) / 16));  // row tiles that hold rows
 
-  const int slot = (r * 4 + (q ^ (r >> 2))) * 16;  // where chunk q of a tile's row r lies
+  const int slot = (r * 4 + (q ^ swizzle4(r))) * 16;  // where chunk q of a tile's row r lies
 
   // The loop over the steps, for the row tiles of this wave that hold rows: known
   // when compiled, so that no branch keeps the reads of one row tile from running
@@ -710,12 +915,26 @@ int launch_tile(const MxArgs& a, int max_tiles, hipStream_t st) {
 
 }  // namespace
 
+namespace {
+
+// Reductions of whole steps of 128, scales that a lane can fetch four at a time,
+// components within 32-bit offsets of their slot: what the streamed and the large
+// tiles need.
+bool mx_aligned(const pmoe_geom* g) {
+  if (g->hidden % 128 || g->inter % 128) return false;
+  const int comps[] = {PMOE_GATE_S, PMOE_UP_S, PMOE_DOWN_S};
+  for (int c : comps)
+    if (g->off[c] % 4 || g->off[c] < 0 ||
+        g->off[c] + int64_t(g->hidden) * g->inter / kMxGroup >= int64_t(1) << 31)
+      return false;
+  return true;
+}
+
+}  // namespace
+
 int mx_tile_rows(const pmoe_geom* g, int n, int kk, int n_experts) {
   const char* v = getenv("PMOE_MX_TILE");
-  // whole steps, and scales that a lane can fetch four at a time
-  if (g->hidden % 128 || g->inter % 128 ||
-      (g->off[PMOE_GATE_S] | g->off[PMOE_UP_S] | g->off[PMOE_DOWN_S]) % 4)
-    return kSmallRows;
+  if (!mx_aligned(g)) return kSmallRows;
   // the tokens' pieces within the large tiles' 32-bit offsets
   if (int64_t(n) * mx_steps(g->hidden) * kMxStepPair >= int64_t(1) << 32) return kSmallRows;
   if (v && v[0] == '0') return kSmallRows;
@@ -734,6 +953,7 @@ int mx_experts(const MxPlan& p, hipStream_t st) {
     PMOE_LAUNCH_CHECK("mx_split_kernel");
   }
   const bool large = p.tile_rows == kTileRows;
+  const bool stream = mx_aligned(g);
   MxArgs a{};
   a.slab = p.slab;
   a.expert_bytes = g->expert_bytes;
@@ -747,8 +967,9 @@ int mx_experts(const MxPlan& p, hipStream_t st) {
   a.cols = g->hidden;
   a.pair = p.xpair, a.third = p.xthird, a.ascale = p.xscale, a.asteps = p.xsteps;
   a.hpair = p.hpair, a.hscale = p.hscale;
-  if (int rc = large ? launch_tile<true, false>(a, p.max_tiles, st)
-                     : launch_small<true, false>(a, p.max_tiles, st))
+  if (int rc = large    ? launch_tile<true, false>(a, p.max_tiles, st)
+               : stream ? launch_stream<true, false>(a, p.max_tiles, st)
+                        : launch_small<true, false>(a, p.max_tiles, st))
     return rc;
   a.w0 = g->off[PMOE_DOWN_W], a.s0 = g->off[PMOE_DOWN_S];
   a.features = g->hidden;
@@ -757,10 +978,12 @@ int mx_experts(const MxPlan& p, hipStream_t st) {
   a.y = p.y;
   a.yscale = p.yscale;
   if (p.yscale)
-    return large ? launch_tile<false, true>(a, p.max_tiles, st)
-                 : launch_small<false, true>(a, p.max_tiles, st);
-  return large ? launch_tile<false, false>(a, p.max_tiles, st)
-               : launch_small<false, false>(a, p.max_tiles, st);
+    return large    ? launch_tile<false, true>(a, p.max_tiles, st)
+           : stream ? launch_stream<false, true>(a, p.max_tiles, st)
+                    : launch_small<false, true>(a, p.max_tiles, st);
+  return large    ? launch_tile<false, false>(a, p.max_tiles, st)
+         : stream ? launch_stream<false, false>(a, p.max_tiles, st)
+                  : launch_small<false, false>(a, p.max_tiles, st);
 }
 
 int mx_combine(const uint16_t* y, const uint8_t* yscale, const float* w, const int32_t* inv,
