@@ -53,6 +53,7 @@ struct MoeWs {
   uint8_t *xpair = nullptr, *xthird = nullptr, *xscale = nullptr;
   uint16_t* xsteps = nullptr;
   uint8_t *hpair = nullptr, *hscale = nullptr;
+  float* h32 = nullptr;       // a single token's intermediate
   uint8_t* yscale = nullptr;  // of the slot outputs that the combine reads
 };
 
@@ -97,6 +98,7 @@ size_t carve(const pmoe_geom* g, int n, int k, int shared, int n_experts, void* 
     t.hpair = c.take<uint8_t>(hs * kMxStepPair);
     t.hscale = c.take<uint8_t>(rows * mx_scale_row(g->inter));
     t.y = reinterpret_cast<float*>(c.take<uint16_t>(rows * g->hidden));
+    t.h32 = n == 1 ? c.take<float>(rows * g->inter) : nullptr;
     t.yscale = c.take<uint8_t>(rows * (g->hidden / kMxGroup));
   } else {
     t.h = c.take<uint16_t>(rows * g->inter);
@@ -512,6 +514,9 @@ int experts_and_combine(const pmoe_geom* g, const uint8_t* slab, const int32_t* 
                         uint16_t* out, const MoeWs& w, hipStream_t st) {
   const int shared = shared_slot >= 0 ? 1 : 0;
   const int kk = k + shared;
+  if (n == 1 && is_mx(g) && mx_one_covers(g))
+    return mx_one(g, slab, table, n_experts, x, inds, wts, k, shared_slot, shared_gate,
+                  w.shared_logit, w.order, w.h32, out, st);
   if (n == 1 && k == kXcdCount && !is_mx(g) && !(shared && shared_gate)) {
     // one token, eight columns: the expert-per-XCD launch (same outputs)
     GemvArgs gu{};
@@ -622,6 +627,10 @@ extern "C" int pmoe_switch_glu(const pmoe_geom* g, const void* slab, const int32
   MoeWs w;
   pmoe::carve(g, n, k, 0, n_experts, ws, &w);
   hipStream_t st = static_cast<hipStream_t>(stream);
+  if (n == 1 && pmoe::is_mx(g) && pmoe::mx_one_covers(g))
+    return pmoe::mx_one(g, static_cast<const uint8_t*>(slab), table, n_experts,
+                        static_cast<const uint16_t*>(x), inds, nullptr, k, -1, nullptr, nullptr,
+                        w.order, w.h32, static_cast<uint16_t*>(y), st);
   rc = pmoe::run_experts(g, static_cast<const uint8_t*>(slab), table, n_experts, -1,
                          static_cast<const uint16_t*>(x), inds, n, k, k, n * k, w, y, 0, st);
   if (rc) return rc;

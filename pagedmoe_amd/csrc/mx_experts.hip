@@ -541,6 +541,304 @@ int launch_stream(const MxArgs& a, int max_tiles, hipStream_t st) {
   return PMOE_OK;
 }
 
+// ---------------------------------------------------------------- one token
+
+constexpr int kOneCols = 16;   // features a block
+constexpr int kOneBatch = 3;   // (column, stretch) items of the down projection in flight a wave
+
+struct MxOne {
+  const uint8_t* slab;
+  int64_t expert_bytes;
+  const int32_t* table;
+  int n_experts;
+  const int32_t* ids;   // [k]
+  const float* wts;     // [k]
+  int k, kk, shared_slot;
+  const uint16_t* shared_gate;  // or null
+  float* shared_logit;
+  int32_t* slots;       // [kk], found by the first launch for the second
+  int64_t w0, s0, w1, s1, wd, sd;
+  const uint16_t* x;
+  int hidden, inter;
+  float* h;             // fp32 [kk, inter]
+  uint16_t* out;        // bf16: [hidden], or [kk, hidden] uncombined
+};
+
+// Slot of column c, -1 where nothing is held.
+__device__ __forceinline__ int one_slot(const MxOne& a, int c) {
+  if (c >= a.k) return a.shared_slot;
+  const int e = a.ids[c];
+  return e >= 0 && e < a.n_experts ? a.table[e] : -1;
+}
+
+// 16 rows x 512 values of a projection into LDS at `to`: 16 lanes side by side on
+// a row's 256 bytes, 4 rows an instruction; then the rows' scales, 4 words each,
+// at to + 4096 (word i of row r at 64 i + 4 r).  In stretch j of `groups` groups,
+// fetched by one wave.
+__device__ __forceinline__ void one_fetch(uint32_t to, const uint8_t* w, const uint8_t* s,
+                                          uint32_t row_bytes, int groups, int j, int lane) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = 4 * i + (lane >> 4);
+    const int p = (lane & 15) ^ swizzle16(row);
+    if (16 * j + p < groups)
+      dma16(to + i * 1024, uint32_t(lane >> 4) * row_bytes + p * 16,
+            w + size_t(4 * i) * row_bytes + j * 256);
+  }
+  const int r = lane & 15, i = lane >> 4;
+  if (16 * j + 4 * i < groups) dma4(to + 4096, uint32_t(r) * groups + 4 * i, s + 16 * j);
+}
+constexpr int kOneFetch = 4096 + 256;
+// A stretch's pieces in LDS: 16 groups of 64 bytes (p0 and p1 48), their scales
+// behind them.
+constexpr int kOnePieces = 16 * 64 + 16;
+// LDS of an item: whole 256 bytes
+constexpr int kOneItem = (kOneFetch + kOnePieces + 255) / 256 * 256;
+
+__device__ __forceinline__ void one_put(uint8_t* to, int g, u32x6 p0, u32x6 p1, uint4 p2) {
+  uint4* d = reinterpret_cast<uint4*>(to + g * 64);
+  d[0] = make_uint4(p0[0], p0[1], p0[2], p0[3]);
+  d[1] = make_uint4(p0[4], p0[5], p1[0], p1[1]);
+  d[2] = make_uint4(p1[2], p1[3], p1[4], p1[5]);
+  d[3] = p2;
+}
+
+// acc += 16 rows of weights at `w` (one_fetch) times a stretch's pieces.
+__device__ __forceinline__ void one_mma(f32x4& acc, const uint8_t* w, const uint8_t* pieces,
+                                        int groups_in, int lane) {
+  const int r = lane & 15, q = lane >> 4;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (4 * i >= groups_in) break;  // whole steps of 128
+    const int p = 4 * i + q;
+    const uint4 v = *reinterpret_cast<const uint4*>(w + (r * 16 + (p ^ swizzle16(r))) * 16);
+    const int sw = w[4096 + 64 * i + 4 * r + q];
+    const uint4* src = reinterpret_cast<const uint4*>(pieces + p * 64);
+    const uint4 c0 = src[0], c1 = src[1], c2 = src[2];
+    const int sa = pieces[16 * 64 + p];
+    const uint32_t b0[6] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y};
+    const uint32_t b1[6] = {c1.z, c1.w, c2.x, c2.y, c2.z, c2.w};
+    mx_mma(acc, v, sw, b0, sa);
+    mx_mma(acc, v, sw, b1, sa - kMxInterShift);
+  }
+}
+
+// h[c, f] = silu(gate) * up for 32 features of one column, the weights streamed as
+// in mx_stream_kernel.  Each wave splits its own stretches of x into pieces, a
+// lane a group, while the slot is looked up and its first weights are on their
+// way.  All 16 columns of the products hold the same row.
+__global__ __launch_bounds__(64 * kMaxWaves, 4) void mx_one_gateup_kernel(const MxOne a,
+                                                                          int wave_lds) {
+  extern __shared__ __attribute__((aligned(1024))) uint8_t dyn[];
+  constexpr int NF = 4, kCols = kStreamRows / 2;
+  const int c = blockIdx.y, fb = blockIdx.x;
+  const int waves = blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int r = lane & 15, q = lane >> 4;
+  const int groups = a.hidden / kMxGroup, steps = groups / kMxStepGroups;
+  uint8_t* own = dyn + wave * wave_lds;
+  uint8_t* pieces = own + kStreamWave;  // [round][8 groups][64 bytes], then their scales
+  const int rounds = (steps + 2 * waves - 1) / (2 * waves);
+  uint8_t* pscale = pieces + rounds * 8 * 64;
+
+  // lane 8 i + k: group k of this wave's i-th step of 256
+  const int mine = 8 * (wave + (lane >> 3) * waves) + (lane & 7);
+  const bool has = (lane >> 3) < rounds && mine < groups;
+  uint4 xin[4];
+  if (has) {
+    const uint4* src = reinterpret_cast<const uint4*>(a.x + size_t(mine) * kMxGroup);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) xin[i] = src[i];
+  }
+  const int slot = one_slot(a, c);
+  if (fb == 0 && threadIdx.x == 0) a.slots[c] = slot;
+  if (slot >= 0) {
+    const uint8_t* base = a.slab + size_t(slot) * size_t(a.expert_bytes);
+    const uint32_t row_bytes = a.hidden / 2;
+    const uint8_t* wbase[NF];
+#pragma unroll
+    for (int f = 0; f < NF; ++f)
+      wbase[f] = base + (f > 1 ? a.w1 : a.w0) + size_t(fb * kCols + 16 * (f & 1)) * row_bytes;
+    const int lrow = lane >> 3;
+    const int lp[2] = {(lane & 7) ^ swizzle8(lrow), (lane & 7) ^ swizzle8(lrow + 8)};
+    const uint32_t s_off =
+        uint32_t(q > 1 ? a.s1 : a.s0) + uint32_t(fb * kCols + 16 * (q & 1) + r) * groups;
+    const uint32_t own_lds = __builtin_amdgcn_readfirstlane(
+        uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)own)));
+    const auto fetch = [&](int j) {
+      const bool two = 2 * j + 1 < steps;
+#pragma unroll
+      for (int f = 0; f < NF; ++f)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (two || lp[i] < 4)
+            dma16(own_lds + f * 2048 + i * 1024, lrow * row_bytes + lp[i] * 16,
+                  wbase[f] + size_t(8 * i) * row_bytes + j * 128);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (i == 0 || two) dma4(own_lds + NF * 2048 + i * 256, s_off + (2 * j + i) * 4, base);
+    };
+    if (2 * wave < steps) fetch(wave);
+    if (has) {
+      float v[32];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t t[4] = {xin[i].x, xin[i].y, xin[i].z, xin[i].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          v[8 * i + 2 * k] = bf16lo(t[k]), v[8 * i + 2 * k + 1] = bf16hi(t[k]);
+      }
+      int s;
+      u32x6 p0, p1;
+      uint4 p2;
+      mx_split<true>(v, s, p0, p1, p2);
+      one_put(pieces, lane, p0, p1, p2);
+      pscale[lane] = uint8_t(s);
+    }
+    f32x4 acc[NF];
+#pragma unroll
+    for (int f = 0; f < NF; ++f) acc[f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    int round = 0;
+    for (int j = wave; 2 * j < steps; j += waves, ++round) {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (2 * j + i >= steps) break;
+        const int at = (r * 8 + ((4 * i + q) ^ swizzle8(r))) * 16;
+        const int g = round * 8 + 4 * i + q;
+        const uint4* src = reinterpret_cast<const uint4*>(pieces + g * 64);
+        const uint4 c0 = src[0], c1 = src[1], c2 = src[2], d = src[3];
+        const int sa = pscale[g];
+        const uint32_t b0[6] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y};
+        const uint32_t b1[6] = {c1.z, c1.w, c2.x, c2.y, c2.z, c2.w};
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+          const uint4 w = *reinterpret_cast<const uint4*>(own + f * 2048 + at);
+          const int sw = own[NF * 2048 + i * 256 + (16 * f + r) * 4 + q];
+          mx_mma(acc[f], w, sw, b0, sa);
+          mx_mma(acc[f], w, sw, b1, sa - kMxTokenShift);
+          mx_mma_third(acc[f], w, sw, d, sa);
+        }
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (2 * (j + waves) < steps) fetch(j + waves);
+    }
+    // lanes 16 q: features 16 f + 4 q + i of the gate (f < 2) and up tiles
+    float(*red)[NF * 16] = reinterpret_cast<float(*)[NF * 16]>(dyn);
+    __syncthreads();
+    if (r == 0)
+#pragma unroll
+      for (int f = 0; f < NF; ++f)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) red[wave][16 * f + 4 * q + i] = acc[f][i];
+    __syncthreads();
+    if (threadIdx.x < kCols) {
+      float g = 0.0f, u = 0.0f;
+      for (int w = 0; w < waves; ++w)
+        g += red[w][threadIdx.x], u += red[w][kCols + threadIdx.x];
+      a.h[size_t(c) * a.inter + fb * kCols + threadIdx.x] = silu_fast(g) * u;
+    }
+  }
+  if (a.shared_gate && fb == 0 && c == a.kk - 1) {  // the shared expert's gate logit
+    float sum = 0.0f;
+    for (int i = threadIdx.x; i < a.hidden; i += blockDim.x)
+      sum = __builtin_fmaf(bf16f(a.x[i]), bf16f(a.shared_gate[i]), sum);
+    sum = wave_sum_bfly(sum);
+    float* red = reinterpret_cast<float*>(dyn);
+    __syncthreads();
+    if (lane == 0) red[wave] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      float t = 0.0f;
+      for (int w = 0; w < waves; ++w) t += red[w];
+      *a.shared_logit = t;
+    }
+  }
+}
+
+// 16 features of the down projection.  MIX: of the weighted sum over all columns,
+// in fp32 (each wave adds up its own (column, stretch) items, the waves meet in
+// LDS, always in the same order); otherwise of column blockIdx.y.
+template <bool MIX>
+__global__ __launch_bounds__(64 * kMaxWaves, 2) void mx_one_down_kernel(const MxOne a, int batch) {
+  extern __shared__ __attribute__((aligned(1024))) uint8_t dyn[];
+  const int f0 = blockIdx.x * kOneCols;
+  const int waves = blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int groups = a.inter / kMxGroup;
+  const int stretches = (groups + 15) / 16;
+  const int first = MIX ? 0 : blockIdx.y, columns = MIX ? a.kk : 1;
+  const int items = columns * stretches;
+  const uint32_t row_bytes = a.inter / 2;
+  uint8_t* own = dyn + wave * batch * kOneItem;
+  const uint32_t own_lds = __builtin_amdgcn_readfirstlane(
+      uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)own)));
+  f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int t0 = wave; t0 < items; t0 += waves * batch) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    for (int b = 0; b < batch; ++b) {
+      const int t = t0 + b * waves;
+      if (t >= items) break;
+      const int c = first + t / stretches, j = t % stretches;
+      const int slot = __builtin_amdgcn_readfirstlane(a.slots[c]);
+      if (slot < 0) continue;
+      const uint8_t* base = a.slab + size_t(slot) * size_t(a.expert_bytes);
+      one_fetch(own_lds + b * kOneItem, base + a.wd + size_t(f0) * row_bytes,
+                base + a.sd + size_t(f0) * groups, row_bytes, groups, j, lane);
+    }
+    {  // 16 lanes an item: a group of its column's h each
+      const int b = lane >> 4, t = t0 + b * waves;
+      if (b < batch && t < items) {
+        const int c = first + t / stretches, gi = 16 * (t % stretches) + (lane & 15);
+        if (gi < groups && a.slots[c] >= 0) {
+          const float4* src = reinterpret_cast<const float4*>(a.h + size_t(c) * a.inter + gi * kMxGroup);
+          float v[32];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float4 x = src[i];
+            v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = x.z, v[4 * i + 3] = x.w;
+          }
+          int s;
+          u32x6 p0, p1;
+          uint4 none;
+          mx_split<false>(v, s, p0, p1, none);
+          uint8_t* to = own + b * kOneItem + kOneFetch;
+          one_put(to, lane & 15, p0, p1, none);
+          to[16 * 64 + (lane & 15)] = uint8_t(s);
+        }
+      }
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    for (int b = 0; b < batch; ++b) {
+      const int t = t0 + b * waves;
+      if (t >= items) break;
+      const int c = first + t / stretches, j = t % stretches;
+      if (__builtin_amdgcn_readfirstlane(a.slots[c]) < 0) continue;
+      f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+      one_mma(acc, own + b * kOneItem, own + b * kOneItem + kOneFetch, min(16, groups - 16 * j),
+                     lane);
+      float w = 1.0f;
+      if constexpr (MIX)
+        w = c < a.k ? a.wts[c] : a.shared_gate ? psigmoid(*a.shared_logit) : 1.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[i] = MIX ? __builtin_fmaf(w, acc[i], sum[i]) : sum[i] + acc[i];
+    }
+  }
+  float(*red)[16] = reinterpret_cast<float(*)[16]>(dyn);
+  __syncthreads();
+  if ((lane & 15) == 0)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) red[wave][(lane >> 4) * 4 + i] = sum[i];
+  __syncthreads();
+  if (threadIdx.x < kOneCols) {
+    float v = 0.0f;
+    for (int w = 0; w < waves; ++w) v += red[w][threadIdx.x];
+    a.out[size_t(MIX ? 0 : blockIdx.y) * a.hidden + f0 + threadIdx.x] = f2bf(v);
+  }
+}
+
 // ---------------------------------------------------------------- large tiles
 
 constexpr int kTileRows = 128;    // activation rows a block
@@ -984,6 +1282,59 @@ int mx_experts(const MxPlan& p, hipStream_t st) {
   return large    ? launch_tile<false, false>(a, p.max_tiles, st)
          : stream ? launch_stream<false, false>(a, p.max_tiles, st)
                   : launch_small<false, false>(a, p.max_tiles, st);
+}
+
+// One token: two launches, no dispatch; out bf16 [hidden] combined (wts given), or
+// [kk, hidden].
+bool mx_one_covers(const pmoe_geom* g) { return mx_aligned(g); }
+
+int mx_one(const pmoe_geom* g, const uint8_t* slab, const int32_t* table, int n_experts,
+           const uint16_t* x, const int32_t* ids, const float* wts, int k, int shared_slot,
+           const uint16_t* shared_gate, float* shared_logit, int32_t* slots, float* h,
+           uint16_t* out, hipStream_t st) {
+  MxOne a{};
+  a.slab = slab;
+  a.expert_bytes = g->expert_bytes;
+  a.table = table;
+  a.n_experts = n_experts;
+  a.ids = ids, a.wts = wts;
+  a.k = k, a.kk = k + (shared_slot >= 0 ? 1 : 0);
+  a.shared_slot = shared_slot;
+  a.shared_gate = shared_slot >= 0 ? shared_gate : nullptr;
+  a.shared_logit = shared_logit;
+  a.slots = slots;
+  a.w0 = g->off[PMOE_GATE_W], a.s0 = g->off[PMOE_GATE_S];
+  a.w1 = g->off[PMOE_UP_W], a.s1 = g->off[PMOE_UP_S];
+  a.wd = g->off[PMOE_DOWN_W], a.sd = g->off[PMOE_DOWN_S];
+  a.x = x;
+  a.hidden = g->hidden, a.inter = g->inter;
+  a.h = h, a.out = out;
+  const auto waves_for = [](int items) {
+    const int rounds = (items + kMaxWaves - 1) / kMaxWaves;
+    return (items + rounds - 1) / rounds;
+  };
+  {
+    const int steps = (a.hidden + kStreamStep - 1) / kStreamStep;
+    const int waves = waves_for(steps);
+    const int rounds = (steps + waves - 1) / waves;  // 8192 / 256 / 8 at most: a lane a group
+    const int wave_lds = (kStreamWave + rounds * 8 * (64 + 1) + 255) / 256 * 256;
+    ProfScope prof_scope(K_MX_GATEUP, st);
+    mx_one_gateup_kernel<<<dim3(a.inter / (kStreamRows / 2), a.kk), 64 * waves, waves * wave_lds,
+                           st>>>(a, wave_lds);
+    PMOE_LAUNCH_CHECK("mx_one_gateup_kernel");
+  }
+  const int stretches = (a.inter + kStep - 1) / kStep;
+  const int items = wts ? a.kk * stretches : stretches;
+  const int waves = waves_for(items);
+  const int batch = std::min((items + waves - 1) / waves, kOneBatch);
+  const size_t lds = size_t(waves) * batch * kOneItem;
+  ProfScope prof_scope(K_MX_DOWN, st);
+  if (wts)
+    mx_one_down_kernel<true><<<a.hidden / kOneCols, 64 * waves, lds, st>>>(a, batch);
+  else
+    mx_one_down_kernel<false><<<dim3(a.hidden / kOneCols, a.kk), 64 * waves, lds, st>>>(a, batch);
+  PMOE_LAUNCH_CHECK("mx_one_down_kernel");
+  return PMOE_OK;
 }
 
 int mx_combine(const uint16_t* y, const uint8_t* yscale, const float* w, const int32_t* inv,
