@@ -18,6 +18,7 @@ from ._lib import Geom, RouteCfg, check, lib
 
 _WS: dict = {}
 _MOE_WS: dict = {}
+_WS_BYTES: dict = {}   # workspace bytes by the sizes that they depend on
 # Workspaces handed out before a larger call replaced them.  They are never
 # freed: a HIP graph captured over an earlier call keeps their raw pointers,
 # and a replay must not write into memory torch has given to another tensor.
@@ -27,7 +28,9 @@ _ERR_HOST: dict = {}
 
 
 def _ptr(t):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+    """t's address as the binding's pointer arguments take it (building a
+    ctypes object for it costs as much again)."""
+    return None if t is None else t.data_ptr()
 
 
 def _stream():
@@ -41,10 +44,19 @@ def _stream():
 def _stream_of(t):
     """The current stream for work on t, which must be on the current device
     (launches go there)."""
-    if t.device.index != torch._C._cuda_getDevice():
+    index = t.get_device()
+    if index != torch._C._cuda_getDevice():
         raise ValueError(f"tensors on {t.device}, but the current device is "
                          f"cuda:{torch._C._cuda_getDevice()}: call under torch.cuda.device")
-    return _stream()
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def _fits(t, dtype, shape, index) -> bool:
+    """Whether t is a contiguous tensor of that type and shape on GPU ``index``:
+    the whole check of the usual call, a tenth of the time of the checks one by
+    one that name what is wrong."""
+    return (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape
+            and t.get_device() == index and t.is_contiguous())
 
 
 def _same_device(a, b, name):
@@ -204,13 +216,14 @@ def mx4_quantize(w: torch.Tensor, out=None):
     (q, scales) contiguous tensors to write into (e.g. slab views)."""
     if not isinstance(w, torch.Tensor) or w.dtype not in _DTYPES:
         raise TypeError("w: expected an fp32, bf16 or fp16 tensor")
-    _need(w, w.dtype, "w", 2)
+    if not (w.dim() == 2 and w.is_cuda and w.is_contiguous()):
+        _need(w, w.dtype, "w", 2)
     r, c = w.shape
     if c == 0 or c % 32:
         raise ValueError("columns must be a multiple of the group size, 32")
     if out is None:
-        q = torch.empty((r, c // 8), dtype=torch.int32, device=w.device)
-        s = torch.empty((r, c // 32), dtype=torch.uint8, device=w.device)
+        q = w.new_empty((r, c // 8), dtype=torch.int32)
+        s = w.new_empty((r, c // 32), dtype=torch.uint8)
     else:
         q, s = out
         for t, dt, shape, name in ((q, torch.int32, (r, c // 8), "q"),
@@ -220,8 +233,8 @@ def mx4_quantize(w: torch.Tensor, out=None):
                 raise ValueError(f"{name}: expected {shape}, got {tuple(t.shape)}")
             _same_device(w, t, name)
     if r:
-        check(lib().pmoe_mx4_quantize(_ptr(w), _DTYPES[w.dtype], r, c, _ptr(q), _ptr(s),
-                                      _stream_of(w)), "pmoe_mx4_quantize")
+        check(lib().pmoe_mx4_quantize(w.data_ptr(), _DTYPES[w.dtype], r, c, q.data_ptr(),
+                                      s.data_ptr(), _stream_of(w)), "pmoe_mx4_quantize")
     return q, s
 
 
@@ -229,18 +242,19 @@ def mx4_dequant(q: torch.Tensor, scales: torch.Tensor, dtype=torch.bfloat16) -> 
     """The values [R, C] of microscaled 4-bit words q [R, C/8] and scales
     [R, C/32], rounded once to ``dtype`` (fp32, bf16 or fp16)."""
     _need(q, torch.int32, "q", 2)
-    _need(scales, torch.uint8, "scales", 2)
     if dtype not in _DTYPES:
         raise TypeError("dtype: expected fp32, bf16 or fp16")
     r, c = q.shape[0], q.shape[1] * 8
-    if c == 0 or c % 32 or tuple(scales.shape) != (r, c // 32):
-        raise ValueError(f"scales: expected {(r, c // 32)} for words {tuple(q.shape)} of whole "
-                         f"groups, got {tuple(scales.shape)}")
-    _same_device(q, scales, "scales")
-    out = torch.empty((r, c), dtype=dtype, device=q.device)
+    if not (c and c % 32 == 0 and _fits(scales, torch.uint8, (r, c // 32), q.get_device())):
+        _need(scales, torch.uint8, "scales", 2)
+        if c == 0 or c % 32 or tuple(scales.shape) != (r, c // 32):
+            raise ValueError(f"scales: expected {(r, c // 32)} for words {tuple(q.shape)} of "
+                             f"whole groups, got {tuple(scales.shape)}")
+        _same_device(q, scales, "scales")
+    out = q.new_empty((r, c), dtype=dtype)
     if r:
-        check(lib().pmoe_mx4_dequant(_ptr(q), _ptr(scales), r, c, _DTYPES[dtype], _ptr(out),
-                                     _stream_of(q)), "pmoe_mx4_dequant")
+        check(lib().pmoe_mx4_dequant(q.data_ptr(), scales.data_ptr(), r, c, _DTYPES[dtype],
+                                     out.data_ptr(), _stream_of(q)), "pmoe_mx4_dequant")
     return out
 
 
@@ -252,13 +266,23 @@ def moe_workspace(g: Geom, n: int, k: int, shared: int, n_experts: int, device,
     synchronisation header is zeroed on allocation (pmoe_moe_workspace_init);
     the cached buffer is separate from the dispatch scratch so nothing else
     ever writes the header.  fresh=True returns a new, private buffer."""
-    nb = max(int(lib().pmoe_moe_workspace(ctypes.byref(g), n, k, shared, n_experts)), 256)
+    sizes = (g.hidden, g.inter, g.group, n, k, shared, n_experts)
+    nb = _WS_BYTES.get(sizes)
+    if nb is None:
+        nb = max(int(lib().pmoe_moe_workspace(ctypes.byref(g), n, k, shared, n_experts)), 256)
+        if len(_WS_BYTES) >= 4096:
+            _WS_BYTES.clear()
+        _WS_BYTES[sizes] = nb
     if fresh:
         buf = torch.empty(nb, dtype=torch.uint8, device=device)
         check(lib().pmoe_moe_workspace_init(_ptr(buf), buf.numel(), _stream()),
               "pmoe_moe_workspace_init")
         return buf
-    buf, new = _grown(_MOE_WS, torch.device(device).index or 0, nb, device, "MoE")
+    index = (device if isinstance(device, torch.device) else torch.device(device)).index or 0
+    buf = _MOE_WS.get(index)
+    if buf is not None and buf.numel() >= nb:
+        return buf
+    buf, new = _grown(_MOE_WS, index, nb, device, "MoE")
     if new:
         check(lib().pmoe_moe_workspace_init(_ptr(buf), buf.numel(), _stream()),
               "pmoe_moe_workspace_init")
@@ -352,7 +376,7 @@ def switch_glu(g: Geom, slab: torch.Tensor, table, n_experts: int, x: torch.Tens
     n, k = inds.shape
     if x.shape != (n, g.hidden):
         raise ValueError(f"x must be [{n}, {g.hidden}], got {tuple(x.shape)}")
-    y = torch.empty((n, k, g.hidden), dtype=torch.bfloat16, device=x.device)
+    y = x.new_empty((n, k, g.hidden))
     if n == 0:
         return y
     ws = moe_workspace(g, n, k, 0, n_experts, x.device)
@@ -434,13 +458,15 @@ def block_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     bf16) with weight [D] (fp32 or bf16; 1 + weight with unit_offset), the
     input of a block (pmoe_block_norm)."""
     xd, wd = _stream_dtype(x, "x"), _stream_dtype(weight, "weight")
-    _need(x, x.dtype, "x", 2)
+    if not (x.dim() == 2 and x.is_cuda and x.is_contiguous()):
+        _need(x, x.dtype, "x", 2)
     n, d = x.shape
-    _like(weight, x, (d,), "weight")
-    h = torch.empty((n, d), dtype=torch.bfloat16, device=x.device)
+    if not _fits(weight, weight.dtype, (d,), x.get_device()):
+        _like(weight, x, (d,), "weight")
+    h = x.new_empty((n, d), dtype=torch.bfloat16)
     if n:
-        check(lib().pmoe_block_norm(_ptr(x), xd, _ptr(weight), wd, n, d, float(eps),
-                                    int(bool(unit_offset)), _ptr(h), _stream_of(x)),
+        check(lib().pmoe_block_norm(x.data_ptr(), xd, weight.data_ptr(), wd, n, d, eps,
+                                    1 if unit_offset else 0, h.data_ptr(), _stream_of(x)),
               "pmoe_block_norm")
     return h
 
@@ -462,34 +488,41 @@ def block_join(residual: torch.Tensor, y: torch.Tensor, weights=None, *, shared_
     ``residual`` itself; it overlaps no other input."""
     j = _lib.Join()
     j.stream_dtype = _stream_dtype(residual, "residual")
-    _need(residual, residual.dtype, "residual", 2)
+    if not (residual.dim() == 2 and residual.is_cuda and residual.is_contiguous()):
+        _need(residual, residual.dtype, "residual", 2)
     n, d = residual.shape
-    _need(y, torch.bfloat16, "y")
-    _same_device(residual, y, "y")
+    dev = residual.get_device()
+    bf16 = torch.bfloat16
     if weights is None:
         k = 1
-        _like(y, residual, (n, d), "y")
+        if not _fits(y, bf16, (n, d), dev):
+            _like(y, residual, (n, d), "y", bf16)
     else:
-        if y.dim() != 3:
-            raise ValueError(f"y: expected [N, K, D] with weights, got {tuple(y.shape)}")
+        _need(y, bf16, "y", 3)
         k = y.shape[1]
-        _like(y, residual, (n, k, d), "y")
-        _like(weights, residual, (n, k), "weights", torch.float32)
-    if shared_y is not None:
-        _like(shared_y, residual, (n, d), "shared_y", torch.bfloat16)
+        if not _fits(y, bf16, (n, k, d), dev):
+            _like(y, residual, (n, k, d), "y")
+        if not _fits(weights, torch.float32, (n, k), dev):
+            _like(weights, residual, (n, k), "weights", torch.float32)
+    if shared_y is not None and not _fits(shared_y, bf16, (n, d), dev):
+        _like(shared_y, residual, (n, d), "shared_y", bf16)
     if shared_logit is not None:
         _need(shared_logit, torch.float32, "shared_logit")
         _same_device(residual, shared_logit, "shared_logit")
         if shared_y is None or shared_logit.numel() != n:
             raise ValueError("shared_logit must hold N values, beside shared_y")
-    norms = [(t, name) for t, name in ((post_weight, "post_weight"), (next_weight, "next_weight"))
-             if t is not None]
-    for t, name in norms:
-        j.weight_dtype = _stream_dtype(t, name, norms[0][0].dtype)
-        _like(t, residual, (d,), name)
+    if post_weight is not None:
+        j.weight_dtype = _stream_dtype(post_weight, "post_weight")
+        if not _fits(post_weight, post_weight.dtype, (d,), dev):
+            _like(post_weight, residual, (d,), "post_weight")
+    if next_weight is not None:
+        j.weight_dtype = _stream_dtype(next_weight, "next_weight",
+                                       None if post_weight is None else post_weight.dtype)
+        if not _fits(next_weight, next_weight.dtype, (d,), dev):
+            _like(next_weight, residual, (d,), "next_weight")
     if gate is not None:
         j.gate_dtype = _stream_dtype(gate, "gate")
-        shape = tuple(gate.shape)
+        shape = gate.shape
         if shape == (d,):
             j.gate_kind = _lib.GATE_CHANNEL
         elif shape == (n, 1):
@@ -497,24 +530,22 @@ def block_join(residual: torch.Tensor, y: torch.Tensor, weights=None, *, shared_
         elif shape == (n, d):
             j.gate_kind = _lib.GATE_ELEMENT
         else:
-            raise ValueError(f"gate: expected {(d,)}, {(n, 1)} or {(n, d)}, got {shape}")
-        _like(gate, residual, shape, "gate")
-    j.gate_sigmoid = int(bool(gate_sigmoid))
-    j.unit_offset = int(bool(unit_offset))
-    j.residual_scale, j.branch_scale = float(residual_scale), float(branch_scale)
-    j.eps = float(eps)
+            raise ValueError(f"gate: expected {(d,)}, {(n, 1)} or {(n, d)}, got {tuple(shape)}")
+        if not _fits(gate, gate.dtype, shape, dev):
+            _like(gate, residual, shape, "gate")
+    j.gate_sigmoid = 1 if gate_sigmoid else 0
+    j.unit_offset = 1 if unit_offset else 0
+    j.residual_scale, j.branch_scale, j.eps = residual_scale, branch_scale, eps
     if out is None:
         out = torch.empty_like(residual)
-    else:
+    elif not _fits(out, residual.dtype, (n, d), dev):
         _like(out, residual, (n, d), "out", residual.dtype)
-    h = None
-    if next_weight is not None:
-        h = torch.empty((n, d), dtype=torch.bfloat16, device=residual.device)
+    h = residual.new_empty((n, d), dtype=bf16) if next_weight is not None else None
     if n:
         check(lib().pmoe_block_join(
-            ctypes.byref(j), _ptr(residual), _ptr(y), _ptr(weights), _ptr(shared_y),
+            ctypes.byref(j), residual.data_ptr(), y.data_ptr(), _ptr(weights), _ptr(shared_y),
             _ptr(shared_logit), _ptr(post_weight), _ptr(gate), _ptr(next_weight), n, k, d,
-            _ptr(out), _ptr(h), _stream_of(residual)), "pmoe_block_join")
+            out.data_ptr(), _ptr(h), _stream_of(residual)), "pmoe_block_join")
     return out, h
 
 
