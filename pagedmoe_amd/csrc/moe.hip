@@ -300,6 +300,33 @@ bool stream_wanted(const pmoe_geom* g, const uint8_t* slab, int n, int kk, int n
   return (rows - distinct) * double(g->expert_bytes) >= double((four ? 100 : 64) * mib);
 }
 
+// The microscaled experts of n tokens with kk columns: into w.y as mx_combine
+// reads them, or into y as the seam's rows.
+int run_mx(const pmoe_geom* g, const uint8_t* slab, const int32_t* table, int n_experts,
+           int shared_slot, const uint16_t* shared_gate, const uint16_t* x, const int32_t* inds,
+           int n, int k, int kk, const MoeWs& w, uint16_t* y, hipStream_t st) {
+  const int64_t rows = int64_t(n) * kk;
+  PMOE_REQUIRE(rows < int64_t(1) << 31, "experts: too many rows for one call");
+  const int n_ids = n_experts + (kk > k ? 1 : 0);
+  MxPlan p{};
+  p.geom = g, p.slab = slab, p.table = table;
+  p.n_experts = n_experts, p.shared_slot = shared_slot;
+  p.x = x, p.ids = inds;
+  p.n = n, p.k = k, p.kk = kk;
+  p.shared_gate = shared_gate, p.shared_logit = w.shared_logit;
+  p.order = w.order, p.counts = w.counts, p.offsets = w.offsets, p.inv = w.inv;
+  p.active = w.active, p.n_active = w.n_active;
+  p.tile_rows = mx_tile_rows(g, n, kk, n_experts);
+  p.tiles = w.tiles, p.n_tiles = w.n_tiles;
+  p.max_tiles = int(rows / p.tile_rows + std::min<int64_t>(rows, n_ids)) + 1;
+  p.dws = w.dws, p.dws_bytes = w.dws_bytes;
+  p.xpair = w.xpair, p.xthird = w.xthird, p.xscale = w.xscale, p.xsteps = w.xsteps;
+  p.hpair = w.hpair, p.hscale = w.hscale;
+  p.y = y ? y : reinterpret_cast<uint16_t*>(w.y);
+  p.yscale = y ? nullptr : w.yscale;
+  return mx_experts(p, st);
+}
+
 // Dispatch + the three projections (+ SwiGLU) for rows = n*kk flat rows.
 // y receives [rows, hidden] (f32 when y_f32, else bf16).
 int run_experts(const pmoe_geom* g, const uint8_t* slab, const int32_t* table, int n_experts,
@@ -307,21 +334,6 @@ int run_experts(const pmoe_geom* g, const uint8_t* slab, const int32_t* table, i
                 int max_rows_per_expert, const MoeWs& w, void* y, int y_f32, hipStream_t st) {
   const int rows = n * kk;
   const int n_ids = n_experts + (kk > k ? 1 : 0);
-  if (is_mx(g)) {
-    const int tm = mx_tile_rows(g, n, kk, n_experts);
-    if (int rc = dispatch_ext(inds, rows, k, kk, n_ids, w.order, w.counts, w.offsets, w.inv,
-                              w.active, w.n_active, tm, w.tiles, w.n_tiles, table, shared_slot,
-                              w.dws, w.dws_bytes, st))
-      return rc;
-    MxPlan p{};
-    p.geom = g, p.slab = slab, p.x = x, p.n = n, p.kk = kk;
-    p.order = w.order, p.tile_rows = tm, p.tiles = w.tiles, p.n_tiles = w.n_tiles;
-    p.max_tiles = rows / tm + std::min(rows, n_ids) + 1;
-    p.xpair = w.xpair, p.xthird = w.xthird, p.xscale = w.xscale, p.xsteps = w.xsteps;
-    p.hpair = w.hpair, p.hscale = w.hscale, p.y = static_cast<uint16_t*>(y);
-    p.yscale = y == w.y ? w.yscale : nullptr;
-    return mx_experts(p, st);
-  }
   const bool stream = stream_wanted(g, slab, n, kk, n_experts, n_ids);
   const bool prefill = !stream && prefill_wanted(g, n, kk, n_ids);
   const int tm = stream ? stream_tile_rows() : prefill ? prefill_tile_rows(n, kk, n_experts) : 0;
@@ -514,10 +526,19 @@ int experts_and_combine(const pmoe_geom* g, const uint8_t* slab, const int32_t* 
                         uint16_t* out, const MoeWs& w, hipStream_t st) {
   const int shared = shared_slot >= 0 ? 1 : 0;
   const int kk = k + shared;
-  if (n == 1 && is_mx(g) && mx_one_covers(g))
-    return mx_one(g, slab, table, n_experts, x, inds, wts, k, shared_slot, shared_gate,
+  if (is_mx(g)) {
+    const uint16_t* gate = shared ? shared_gate : nullptr;
+    if (n > 1 || !mx_one_covers(g)) {
+      if (int rc = run_mx(g, slab, table, n_experts, shared_slot, gate, x, inds, n, k, kk, w,
+                          nullptr, st))
+        return rc;
+      return mx_combine(reinterpret_cast<const uint16_t*>(w.y), w.yscale, wts, w.inv,
+                        gate ? w.shared_logit : nullptr, n, k, kk, g->hidden, out, st);
+    }
+    return mx_one(g, slab, table, n_experts, x, inds, wts, k, shared_slot, gate,
                   w.shared_logit, w.order, w.h32, out, st);
-  if (n == 1 && k == kXcdCount && !is_mx(g) && !(shared && shared_gate)) {
+  }
+  if (n == 1 && k == kXcdCount && !(shared && shared_gate)) {
     // one token, eight columns: the expert-per-XCD launch (same outputs)
     GemvArgs gu{};
     gu.slab = slab;
@@ -550,9 +571,6 @@ int experts_and_combine(const pmoe_geom* g, const uint8_t* slab, const int32_t* 
     if (rc) return rc;
     sl = w.shared_logit;
   }
-  if (is_mx(g))
-    return mx_combine(reinterpret_cast<const uint16_t*>(w.y), w.yscale, wts, w.inv, sl, n, k, kk,
-                      g->hidden, out, st);
   dim3 grid((g->hidden / 8 + 255) / 256, n);
   ProfScope prof_scope(K_COMBINE, st);
   combine_kernel<<<grid, 256, 0, st>>>(reinterpret_cast<const uint16_t*>(w.y), wts, w.inv, sl,
@@ -631,6 +649,10 @@ extern "C" int pmoe_switch_glu(const pmoe_geom* g, const void* slab, const int32
     return pmoe::mx_one(g, static_cast<const uint8_t*>(slab), table, n_experts,
                         static_cast<const uint16_t*>(x), inds, nullptr, k, -1, nullptr, nullptr,
                         w.order, w.h32, static_cast<uint16_t*>(y), st);
+  if (pmoe::is_mx(g))
+    return pmoe::run_mx(g, static_cast<const uint8_t*>(slab), table, n_experts, -1, nullptr,
+                        static_cast<const uint16_t*>(x), inds, n, k, k, w,
+                        static_cast<uint16_t*>(y), st);
   rc = pmoe::run_experts(g, static_cast<const uint8_t*>(slab), table, n_experts, -1,
                          static_cast<const uint16_t*>(x), inds, n, k, k, n * k, w, y, 0, st);
   if (rc) return rc;

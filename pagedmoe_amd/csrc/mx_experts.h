@@ -31,26 +31,35 @@ struct MxArgs {
 struct MxPlan {
   const pmoe_geom* geom;
   const uint8_t* slab;
-  const uint16_t* x;  // bf16 [n, hidden]
-  int n, kk;
-  const int32_t* order;
+  const int32_t* table;
+  int n_experts, shared_slot;
+  const uint16_t* x;   // bf16 [n, hidden]
+  const int32_t* ids;  // [n, k]
+  int n, k, kk;
+  const uint16_t* shared_gate;  // or null; shared_logit[n] receives x . shared_gate
+  float* shared_logit;
+  // scratch: the dispatch's (pmoe_kernels.h) ...
+  int32_t *order, *counts, *offsets, *inv, *active, *n_active;
   int tile_rows;  // of the tile list
-  const int4* tiles;
-  const int32_t* n_tiles;
+  int4* tiles;
+  int32_t* n_tiles;
   int max_tiles;
-  // scratch: the tokens' pieces, the sorted rows' intermediate
+  void* dws;
+  size_t dws_bytes;
+  // ... the tokens' pieces, the sorted rows' intermediate
   uint8_t *xpair, *xthird, *xscale;
   uint16_t* xsteps;  // [n, 4]
   uint8_t *hpair, *hscale;
-  uint16_t* y;      // [n * kk, hidden]: bf16, or fp16 under yscale where that is not null
+  // [n * kk, hidden]: fp16 under yscale, for mx_combine, or (yscale null) the seam's
+  // bf16 rows, those of dropped ids zero
+  uint16_t* y;
   uint8_t* yscale;  // [n * kk, hidden / 32]
 };
 
 // Rows of the dispatch's tiles for such a call, and the fewest that any has.
 int mx_tile_rows(const pmoe_geom* g, int n, int kk, int n_experts);
 int mx_min_tile_rows();
-// Split, gate/up, down over the dispatch's tiles; rows whose expert is not
-// resident come out zero.
+// Dispatch, split, gate/up, down; rows whose expert is not resident come out zero.
 int mx_experts(const MxPlan& p, hipStream_t st);
 // One token in two launches, without a dispatch: out bf16 [hidden] combined (wts
 // given) or [k, hidden].  slots [k + 1], h fp32 [k + 1, inter]: scratch.

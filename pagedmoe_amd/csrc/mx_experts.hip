@@ -16,6 +16,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "dispatch_small.h"
 #include "mx_experts.h"
 #include "mx_pieces.h"
 #include "pmoe_internal.h"
@@ -122,21 +123,28 @@ __global__ __launch_bounds__(256) void mx_combine_kernel(
 
 // ---------------------------------------------------------------- activations
 
-// One lane a group: x bf16 [n, d] into pieces, scales and each token's mask of
-// the 128-wide steps that hold a third piece (16 bits a wave, 4 waves a token).
-__global__ __launch_bounds__(256) void mx_split_kernel(const uint16_t* __restrict__ x, int n,
-                                                       int groups, int steps128, int scale_row,
-                                                       uint8_t* __restrict__ pair,
-                                                       uint8_t* __restrict__ third,
-                                                       uint8_t* __restrict__ scales,
-                                                       uint16_t* __restrict__ steps) {
-  const int token = blockIdx.x;
-  const int g = threadIdx.x;
+struct MxSplit {
+  const uint16_t* x;  // bf16 [n, 32 * groups]
+  int n, groups, steps, scale_row;
+  uint8_t *pair, *third, *scales;
+  uint16_t* masks;              // [n, 4]
+  const uint16_t* shared_gate;  // or null: shared_logit[n] = x . shared_gate
+  float* shared_logit;
+  const int32_t* ids;           // [n, k]
+  int k, n_experts;
+  uint16_t* y;                  // or null: rows [n, k, d] of ids out of range become zero
+};
+
+// A token by 256 threads, a lane a group: its pieces, scales and the mask of the
+// 128-wide steps that hold a third piece (16 bits a wave), the shared expert's gate
+// logit, the zero rows of ids that are dropped.  s_sum: 4 floats of the token's.
+__device__ __forceinline__ void split_token(const MxSplit& a, int token, int g, float* s_sum) {
   bool peak = false;
-  if (g < groups) {
-    const size_t row = size_t(token) * steps128;
+  float dot = 0.0f;
+  if (token < a.n && g < a.groups) {
+    const size_t row = size_t(token) * a.steps;
     const uint4* src =
-        reinterpret_cast<const uint4*>(x + (size_t(token) * groups + g) * kMxGroup);
+        reinterpret_cast<const uint4*>(a.x + (size_t(token) * a.groups + g) * kMxGroup);
     float v[32];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -146,21 +154,67 @@ __global__ __launch_bounds__(256) void mx_split_kernel(const uint16_t* __restric
       for (int j = 0; j < 4; ++j)
         v[8 * i + 2 * j] = bf16lo(w[j]), v[8 * i + 2 * j + 1] = bf16hi(w[j]);
     }
+    if (a.shared_gate)
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        dot = __builtin_fmaf(v[i], bf16f(a.shared_gate[g * kMxGroup + i]), dot);
     int s;
     u32x6 p0, p1;
     uint4 p2;
     peak = mx_split<true>(v, s, p0, p1, p2);
-    mx_store_pair(pair + row * kMxStepPair, g, p0, p1);
-    mx_store_third(third + row * kMxStepThird, g, p2);
-    scales[size_t(token) * scale_row + mx_scale_at(g)] = uint8_t(s);
+    mx_store_pair(a.pair + row * kMxStepPair, g, p0, p1);
+    mx_store_third(a.third + row * kMxStepThird, g, p2);
+    a.scales[size_t(token) * a.scale_row + mx_scale_at(g)] = uint8_t(s);
   }
   const uint64_t m = __ballot(peak);
-  if ((threadIdx.x & 63) == 0) {
+  if (token < a.n && (g & 63) == 0) {
     uint32_t bits = 0;
 #pragma unroll
     for (int i = 0; i < 16; ++i) bits |= (m >> (4 * i) & 15) ? 1u << i : 0u;
-    steps[size_t(token) * 4 + (threadIdx.x >> 6)] = uint16_t(bits);
+    a.masks[size_t(token) * 4 + (g >> 6)] = uint16_t(bits);
   }
+  if (a.shared_gate) {
+    dot = wave_sum_bfly(dot);
+    if ((g & 63) == 0) s_sum[g >> 6] = dot;
+    __syncthreads();
+    if (token < a.n && g == 0) a.shared_logit[token] = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+  }
+  if (a.y && token < a.n) {
+    const int d = a.groups * kMxGroup;
+    for (int c = 0; c < a.k; ++c) {
+      const size_t row = size_t(token) * a.k + c;
+      const int e = a.ids[row];
+      if (e >= 0 && e < a.n_experts) continue;
+      for (int i = g * 8; i < d; i += 256 * 8)
+        *reinterpret_cast<uint4*>(a.y + row * d + i) = make_uint4(0, 0, 0, 0);
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void mx_split_kernel(const MxSplit a) {
+  __shared__ float s_sum[4];
+  split_token(a, blockIdx.x, threadIdx.x, s_sum);
+}
+
+// The dispatch of a small call beside its split: block 0 dispatches, the others
+// take four tokens each.
+struct MxDispatch {
+  IdSrc src;
+  int rows, n_ids;
+  int32_t *order, *counts, *offsets, *inv, *active, *n_active;
+  TileSink tiles;
+};
+
+__global__ __launch_bounds__(1024) void mx_prepare_kernel(const MxSplit a, const MxDispatch d) {
+  __shared__ DispatchLds lds;
+  if (blockIdx.x == 0) {
+    dispatch_small(lds, d.src, d.rows, d.n_ids, d.order, d.counts, d.offsets, d.inv, d.active,
+                   d.n_active, d.tiles);
+    return;
+  }
+  const int quarter = threadIdx.x >> 8;
+  split_token(a, (blockIdx.x - 1) * 4 + quarter, threadIdx.x & 255,
+              reinterpret_cast<float*>(lds.tmp) + 4 * quarter);
 }
 
 // ---------------------------------------------------------------- memory to LDS
@@ -192,7 +246,7 @@ __device__ __forceinline__ int swizzle16(int r) { return (r & 3) << 1 | (r & 8);
 
 // ---------------------------------------------------------------- small tiles
 
-constexpr int kSmallRows = 16;   // activation rows a tile
+constexpr int kFewRows = 16;     // activation rows a tile
 constexpr int kSmallCols = 32;   // features a block (one group of the next product)
 constexpr int kStep = 512;       // reduction that a wave takes at a time
 constexpr int kMaxWaves = 8;
@@ -205,13 +259,13 @@ template <bool DUAL, bool HALF>
 __global__ __launch_bounds__(64 * kMaxWaves) void mx_small_kernel(const MxArgs a) {
   constexpr int NF = DUAL ? 4 : 2;  // 16-feature tiles: gate, gate, up, up
   __shared__ float s_red[kMaxWaves][NF * 4][64];
-  __shared__ float s_h[kSmallRows][kSmallCols + 1];
+  __shared__ float s_h[kFewRows][kSmallCols + 1];
   const int fblocks = a.features / kSmallCols;
   const int t = blockIdx.x / fblocks;
   const int fb = blockIdx.x - t * fblocks;
   if (t >= *a.n_tiles) return;
   const int4 tile = a.tiles[t];  // {slot, first row, rows of the expert, offset}
-  const int m = min(kSmallRows, tile.z - tile.y);
+  const int m = min(kFewRows, tile.z - tile.y);
   const int p0 = tile.w + tile.y;
   const int waves = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -291,7 +345,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void mx_small_kernel(const MxArgs a
     for (int i = 0; i < 4; ++i) s_red[wave][4 * f + i][lane] = acc[f][i];
   __syncthreads();
   // feature c of row s_r: accumulator c % 4 of lane 16 (c % 16 / 4) + row
-  for (int i = threadIdx.x; i < kSmallRows * kSmallCols; i += blockDim.x) {
+  for (int i = threadIdx.x; i < kFewRows * kSmallCols; i += blockDim.x) {
     const int row = i / kSmallCols, c = i % kSmallCols;
     if (row >= m) break;  // whole halves of a wave
     const int src = (c & 15) / 4 * 16 + row;
@@ -367,7 +421,7 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void mx_stream_kernel(const MxAr
   const int fb = blockIdx.x - t * fblocks;
   if (t >= *a.n_tiles) return;
   const int4 tile = a.tiles[t];  // {slot, first row, rows of the expert, offset}
-  const int m = min(kSmallRows, tile.z - tile.y);
+  const int m = min(kFewRows, tile.z - tile.y);
   const int p0 = tile.w + tile.y;
   const int waves = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -486,7 +540,7 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void mx_stream_kernel(const MxAr
 #pragma unroll
     for (int i = 0; i < 4; ++i) red[wave][4 * f + i][lane] = acc[f][i];
   __syncthreads();
-  for (int i = threadIdx.x; i < kSmallRows * kCols; i += blockDim.x) {
+  for (int i = threadIdx.x; i < kFewRows * kCols; i += blockDim.x) {
     const int row = i / kCols, c = i % kCols;
     if (row >= m) break;  // whole halves of a wave
     const int src = (c & 15) / 4 * 16 + row;
@@ -534,7 +588,7 @@ int launch_stream(const MxArgs& a, int max_tiles, hipStream_t st) {
   const int64_t blocks = int64_t(max_tiles) * ((a.features + kCols - 1) / kCols);
   PMOE_REQUIRE(blocks < (int64_t(1) << 31), "experts: too many tiles for one call");
   const size_t lds = std::max<size_t>(size_t(waves) * kStreamWave,
-                                      size_t(waves) * 4096 + kSmallRows * (kCols + 1) * 4);
+                                      size_t(waves) * 4096 + kFewRows * (kCols + 1) * 4);
   ProfScope prof_scope(DUAL ? K_MX_GATEUP : K_MX_DOWN, st);
   mx_stream_kernel<DUAL, HALF><<<unsigned(blocks), 64 * waves, lds, st>>>(a);
   PMOE_LAUNCH_CHECK("mx_stream_kernel");
@@ -1232,22 +1286,45 @@ bool mx_aligned(const pmoe_geom* g) {
 
 int mx_tile_rows(const pmoe_geom* g, int n, int kk, int n_experts) {
   const char* v = getenv("PMOE_MX_TILE");
-  if (!mx_aligned(g)) return kSmallRows;
+  if (!mx_aligned(g)) return kFewRows;
   // the tokens' pieces within the large tiles' 32-bit offsets
-  if (int64_t(n) * mx_steps(g->hidden) * kMxStepPair >= int64_t(1) << 32) return kSmallRows;
-  if (v && v[0] == '0') return kSmallRows;
+  if (int64_t(n) * mx_steps(g->hidden) * kMxStepPair >= int64_t(1) << 32) return kFewRows;
+  if (v && v[0] == '0') return kFewRows;
   if (v && v[0] == '1') return kTileRows;
-  return int64_t(n) * kk >= 16L * n_experts ? kTileRows : kSmallRows;
+  return int64_t(n) * kk >= 16L * n_experts ? kTileRows : kFewRows;
 }
-int mx_min_tile_rows() { return kSmallRows; }
+int mx_min_tile_rows() { return kFewRows; }
 
 int mx_experts(const MxPlan& p, hipStream_t st) {
   const pmoe_geom* g = p.geom;
-  {
+  const bool shared = p.kk > p.k;
+  const int n_ids = p.n_experts + (shared ? 1 : 0), rows = p.n * p.kk;
+  PMOE_REQUIRE(n_ids <= kMaxExperts, "dispatch: experts must be 1..1024");
+  MxSplit sp{};
+  sp.x = p.x;
+  sp.n = p.n, sp.groups = g->hidden / kMxGroup, sp.steps = mx_steps(g->hidden);
+  sp.scale_row = mx_scale_row(g->hidden);
+  sp.pair = p.xpair, sp.third = p.xthird, sp.scales = p.xscale, sp.masks = p.xsteps;
+  sp.shared_gate = p.shared_gate, sp.shared_logit = p.shared_logit;
+  sp.ids = p.ids, sp.k = p.k, sp.n_experts = p.n_experts;
+  sp.y = p.yscale ? nullptr : p.y;
+  if (rows <= kSmallRows) {
+    MxDispatch d{};
+    d.src = IdSrc{p.ids, p.k, p.kk, p.n_experts};
+    d.rows = rows, d.n_ids = n_ids;
+    d.order = p.order, d.counts = p.counts, d.offsets = p.offsets, d.inv = p.inv;
+    d.active = p.active, d.n_active = p.n_active;
+    d.tiles = TileSink{p.tiles, p.n_tiles, p.tile_rows, p.table, p.n_experts, p.shared_slot};
     ProfScope prof_scope(K_MX_SPLIT, st);
-    mx_split_kernel<<<p.n, 256, 0, st>>>(p.x, p.n, g->hidden / kMxGroup, mx_steps(g->hidden),
-                                         mx_scale_row(g->hidden), p.xpair, p.xthird, p.xscale,
-                                         p.xsteps);
+    mx_prepare_kernel<<<1 + (p.n + 3) / 4, 1024, 0, st>>>(sp, d);
+    PMOE_LAUNCH_CHECK("mx_prepare_kernel");
+  } else {
+    if (int rc = dispatch_ext(p.ids, rows, p.k, p.kk, n_ids, p.order, p.counts, p.offsets, p.inv,
+                              p.active, p.n_active, p.tile_rows, p.tiles, p.n_tiles, p.table,
+                              p.shared_slot, p.dws, p.dws_bytes, st))
+      return rc;
+    ProfScope prof_scope(K_MX_SPLIT, st);
+    mx_split_kernel<<<p.n, 256, 0, st>>>(sp);
     PMOE_LAUNCH_CHECK("mx_split_kernel");
   }
   const bool large = p.tile_rows == kTileRows;
