@@ -57,8 +57,8 @@ enum {
  *
  * bits 4 with group 32 is the microscaled format (pmoe_mx4_quantize): scales
  * are u8 [.., cols/32] and the biases components are empty.  Dims are
- * multiples of 32, and the slab, expert_bytes and the weight components'
- * offsets multiples of 16 bytes.  Every entry point that takes a geometry takes
+ * multiples of 32, and the slab, expert_bytes, the weight components' offsets,
+ * x and the outputs lie on 16 bytes.  Every entry point that takes a geometry takes
  * either format.  A row whose activations hold an infinity or a NaN, or whose
  * intermediate leaves fp32, comes out as NaN there. */
 typedef struct {

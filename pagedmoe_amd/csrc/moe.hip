@@ -208,7 +208,9 @@ __global__ __launch_bounds__(256) void zero_dropped_rows_kernel(const int32_t* _
   for (int i = threadIdx.x; i < d; i += 256) y[size_t(r) * d + i] = 0;
 }
 
-int check_geom(const pmoe_geom* g, const void* slab) {
+// rows: what the microscaled kernels read and write 16 bytes at a time (null: none).
+int check_geom(const pmoe_geom* g, const void* slab, const void* x = nullptr,
+               const void* rows = nullptr) {
   PMOE_REQUIRE(g != nullptr, "null geometry");
   PMOE_REQUIRE(g->bits == 4 || g->bits == 6, "geometry: bits must be 4 or 6");
   if (is_mx(g)) {
@@ -219,6 +221,8 @@ int check_geom(const pmoe_geom* g, const void* slab) {
     PMOE_REQUIRE((g->expert_bytes | g->off[PMOE_GATE_W] | g->off[PMOE_UP_W] |
                   g->off[PMOE_DOWN_W]) % 16 == 0 && reinterpret_cast<uintptr_t>(slab) % 16 == 0,
                  "geometry: microscaled weights must lie on 16 bytes");
+    PMOE_REQUIRE((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(rows)) % 16 == 0,
+                 "geometry: x and the outputs of microscaled experts must lie on 16 bytes");
     return PMOE_OK;
   }
   PMOE_REQUIRE(g->group == 64, "geometry: group must be 64");
@@ -520,6 +524,34 @@ int decode_block(const pmoe_geom* g, const pmoe_route_cfg* rc, const uint8_t* sl
   return decode_routed(gu, dn, rt, g->bits, inds_out, w_out, out, w.record, ri, st);
 }
 
+// The routing of a small batch in one launch (decode_block's, without the shared
+// expert's gate), for experts that run apart from it.
+int route_mx(const pmoe_route_cfg* rc, const int32_t* table, const uint16_t* gate_w,
+             const float* score_bias, const float* logit_bias, const uint16_t* x, int n, int d,
+             int shared_slot, int32_t* inds_out, float* w_out, const MoeWs& w, hipStream_t st) {
+  RouteDev rt{};
+  rt.logits = w.logits;
+  rt.ld = rc->n_experts;
+  rt.bias = score_bias;
+  rt.scoring = rc->scoring;
+  rt.n = n;
+  rt.e = rc->n_experts;
+  rt.k = rc->top_k;
+  rt.kk = rc->top_k + (shared_slot >= 0 ? 1 : 0);
+  rt.norm = rc->norm_topk_prob;
+  rt.n_group = rc->n_group;
+  rt.topk_group = rc->topk_group;
+  rt.scale = rc->routed_scale;
+  GemvArgs gu{};
+  gu.table = table;
+  gu.n_experts = rc->n_experts;
+  gu.shared_slot = shared_slot;
+  const RouterIn ri{x, gate_w, nullptr, logit_bias, d, w.logits,
+                    reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(w.sync) +
+                                                kRouteArriveOffset)};
+  return decode_route(gu, rt, inds_out, w_out, w.record, ri, st);
+}
+
 int experts_and_combine(const pmoe_geom* g, const uint8_t* slab, const int32_t* table,
                         int n_experts, const uint16_t* x, const int32_t* inds, const float* wts,
                         int n, int k, int shared_slot, const uint16_t* shared_gate, int max_rpe,
@@ -635,7 +667,7 @@ extern "C" int pmoe_switch_glu(const pmoe_geom* g, const void* slab, const int32
                                int n_experts, const void* x, const int32_t* inds, int n, int k,
                                void* y, void* ws, size_t ws_bytes, void* stream) {
   pmoe::clear_error();
-  int rc = pmoe::check_geom(g, slab);
+  int rc = pmoe::check_geom(g, slab, x, y);
   if (rc) return rc;
   PMOE_REQUIRE(slab && table && x && inds && y, "switch_glu: null pointer");
   PMOE_REQUIRE(n >= 0 && k > 0 && n_experts > 0 && n_experts <= 1023, "switch_glu: bad shape");
@@ -669,7 +701,7 @@ extern "C" int pmoe_moe_experts(const pmoe_geom* g, const void* slab, const int3
                                 const void* shared_gate, void* out, void* ws, size_t ws_bytes,
                                 void* stream) {
   pmoe::clear_error();
-  int rc = pmoe::check_geom(g, slab);
+  int rc = pmoe::check_geom(g, slab, x, out);
   if (rc) return rc;
   PMOE_REQUIRE(slab && table && x && inds && weights && out, "moe_experts: null pointer");
   PMOE_REQUIRE(n >= 0 && k > 0 && n_experts > 0 && n_experts <= 1023, "moe_experts: bad shape");
@@ -691,7 +723,7 @@ extern "C" int pmoe_moe_block(const pmoe_geom* g, const pmoe_route_cfg* rc_cfg, 
                               const void* shared_gate, void* out, int32_t* inds_out,
                               float* weights_out, void* ws, size_t ws_bytes, void* stream) {
   pmoe::clear_error();
-  int rc = pmoe::check_geom(g, slab);
+  int rc = pmoe::check_geom(g, slab, x, out);
   if (rc) return rc;
   PMOE_REQUIRE(rc_cfg != nullptr, "moe_block: null routing config");
   PMOE_REQUIRE(slab && table && gate_w && x && out && inds_out && weights_out,
@@ -709,14 +741,24 @@ extern "C" int pmoe_moe_block(const pmoe_geom* g, const pmoe_route_cfg* rc_cfg, 
   hipStream_t st = static_cast<hipStream_t>(stream);
   const uint16_t* xb = static_cast<const uint16_t*>(x);
   const int kk = k + shared;
-  const bool decode = n * kk <= pmoe::kRouteMaxRows && e + 1 <= pmoe::kRouteMaxIds &&
-                      k <= pmoe::kRouteMaxK && !pmoe::is_mx(g) &&
-                      !pmoe::prefill_wanted(g, n, kk, e + shared) &&
-                      (rc_cfg->scoring == PMOE_SCORE_SOFTMAX ||
-                       (e <= pmoe::kRouteMaxSigE && rc_cfg->topk_group <= 8));
+  const bool routed_at_once = n * kk <= pmoe::kRouteMaxRows && e + 1 <= pmoe::kRouteMaxIds &&
+                              k <= pmoe::kRouteMaxK &&
+                              (rc_cfg->scoring == PMOE_SCORE_SOFTMAX ||
+                               (e <= pmoe::kRouteMaxSigE && rc_cfg->topk_group <= 8));
+  const bool decode =
+      routed_at_once && !pmoe::is_mx(g) && !pmoe::prefill_wanted(g, n, kk, e + shared);
+  if (rc_cfg->scoring == PMOE_SCORE_SIGMOID)
+    PMOE_REQUIRE(score_bias != nullptr, "moe_block: sigmoid scoring needs score_bias");
+  if (pmoe::is_mx(g) && routed_at_once) {
+    rc = pmoe::route_mx(rc_cfg, table, static_cast<const uint16_t*>(gate_w), score_bias,
+                        logit_bias, xb, n, g->hidden, shared_slot, inds_out, weights_out, w, st);
+    if (rc) return rc;
+    return pmoe::experts_and_combine(g, static_cast<const uint8_t*>(slab), table, e, xb, inds_out,
+                                     weights_out, n, k, shared_slot,
+                                     static_cast<const uint16_t*>(shared_gate), n,
+                                     static_cast<uint16_t*>(out), w, st);
+  }
   if (decode) {
-    if (rc_cfg->scoring == PMOE_SCORE_SIGMOID)
-      PMOE_REQUIRE(score_bias != nullptr, "moe_block: sigmoid scoring needs score_bias");
     return pmoe::decode_block(g, rc_cfg, static_cast<const uint8_t*>(slab), table,
                               static_cast<const uint16_t*>(gate_w), score_bias, logit_bias, xb, n,
                               shared_slot, static_cast<const uint16_t*>(shared_gate),

@@ -1284,14 +1284,28 @@ bool mx_aligned(const pmoe_geom* g) {
 
 }  // namespace
 
+// Rows of a tile: 16 (streamed tiles, which read an expert's weights again for
+// every 16 rows) or 128.  The large tiles pay from 12 rows an expert where their
+// blocks, one a CU at a time, fill the GPU one and a half times, and from
+// proportionally more where they do not.  us, gate/up + down, 16 / 128 rows a tile:
+//   4096x1536, 128 experts  9 rows an expert 301 / 319, 13: 343 / 322, 25: 523 / 344
+//   2048x512, 512 experts   9: 225 / 258, 13: 259 / 266, 17: 306 / 272
+//   7168x2048, 385 experts  7: 1960 / 1993, 12: 2324 / 2135
+//   2048x768, 128 experts   9: 94 / 106, 13: 105 / 107, 19: 134 / 114
+//   1024x512, 32 experts    50: 37 / 46, 75: 47 / 48, 100: 55 / 50
+//   4096x1536, 8 experts    50: 74 / 97, 100: 121 / 103
+// PMOE_MX_TILE=0 / 1 pins 16 / 128 where the shape allows it (read per call).
 int mx_tile_rows(const pmoe_geom* g, int n, int kk, int n_experts) {
-  const char* v = getenv("PMOE_MX_TILE");
   if (!mx_aligned(g)) return kFewRows;
   // the tokens' pieces within the large tiles' 32-bit offsets
   if (int64_t(n) * mx_steps(g->hidden) * kMxStepPair >= int64_t(1) << 32) return kFewRows;
-  if (v && v[0] == '0') return kFewRows;
-  if (v && v[0] == '1') return kTileRows;
-  return int64_t(n) * kk >= 16L * n_experts ? kTileRows : kFewRows;
+  const char* v = getenv("PMOE_MX_TILE");
+  if (v && (v[0] == '0' || v[0] == '1')) return v[0] == '1' ? kTileRows : kFewRows;
+  const int64_t rows = int64_t(n) * kk;
+  const int64_t blocks =
+      (n_experts + rows / kTileRows) * ((g->inter + kTileCols / 2 - 1) / (kTileCols / 2));
+  constexpr int64_t kFull = 384;
+  return rows * std::min(blocks, kFull) >= 12 * kFull * n_experts ? kTileRows : kFewRows;
 }
 int mx_min_tile_rows() { return kFewRows; }
 

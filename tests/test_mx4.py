@@ -106,6 +106,22 @@ def test_expert_entries_refuse_bad_geometries(change):
                             1 << 40, None) == -1
 
 
+@pytest.mark.parametrize("which", ["x", "out"])
+def test_expert_entries_refuse_rows_off_16_bytes(which):
+    L = _lib.lib()
+    g = _lib.geom(1024, 512, 4, 32)
+    p = ctypes.byref(g)
+    x, out = (ctypes.c_void_p(0x1002 if which == n else 0x1000) for n in ("x", "out"))
+    rc = _lib.RouteCfg()
+    rc.n_experts, rc.top_k, rc.routed_scale = 8, 2, 1.0
+    assert L.pmoe_switch_glu(p, D, D, 8, x, D, 1, 2, out, D, 1 << 40, None) == -1
+    assert b"16 bytes" in L.pmoe_last_error()
+    assert L.pmoe_moe_experts(p, D, D, 8, x, D, D, 1, 2, -1, None, out, D, 1 << 40, None) == -1
+    assert L.pmoe_moe_block(p, ctypes.byref(rc), D, D, D, None, None, x, 1, -1, None, out, D, D, D,
+                            1 << 40, None) == -1
+    assert b"16 bytes" in L.pmoe_last_error()
+
+
 def test_expert_entries_refuse_a_small_workspace():
     L = _lib.lib()
     g = _lib.geom(1024, 512, 4, 32)
