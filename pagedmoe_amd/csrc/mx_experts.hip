@@ -28,6 +28,7 @@ namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kFp4 = 4, kFp6 = 2;  // operand formats of the scaled MFMA
 
@@ -89,8 +90,13 @@ __device__ __forceinline__ uint32_t half_wave_max(uint32_t v) {
   return v;
 }
 
+// Slot outputs of this size are written and read past the caches, which would not
+// hold them.
+inline bool past_caches(int64_t values) { return values >= int64_t(128) << 20; }
+
 // out[n] = bf16(fma over k of weight * y, then the shared expert's times 1 or
 // sigmoid(shared_logit[n])), in column order; 8 features a thread.
+template <bool PAST>
 __global__ __launch_bounds__(256) void mx_combine_kernel(
     const uint16_t* __restrict__ y, const uint8_t* __restrict__ yscale,
     const float* __restrict__ w, const int32_t* __restrict__ inv,
@@ -100,19 +106,35 @@ __global__ __launch_bounds__(256) void mx_combine_kernel(
   const int d0 = ((blockIdx.x - n * blocks_row) * 256 + threadIdx.x) * 8;
   if (d0 >= d) return;
   float a[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-  for (int c = 0; c < kk; ++c) {
-    const size_t r = size_t(n) * kk + c;
-    if (inv[r] < 0) continue;  // dropped id: contributes nothing
-    float wt = c < k ? w[size_t(n) * k + c] : shared_logit ? psigmoid(shared_logit[n]) : 1.0f;
-    const float unit = half_unit(yscale[r * (d / kMxGroup) + d0 / kMxGroup]);
-    const uint4 v = *reinterpret_cast<const uint4*>(y + r * d + d0);
-    const uint32_t p[4] = {v.x, v.y, v.z, v.w};
+  constexpr int kBatch = 4;  // columns whose loads are in flight together
+  for (int c0 = 0; c0 < kk; c0 += kBatch) {
+    u32x4 v[kBatch];
+    float wt[kBatch], unit[kBatch];
+    bool in[kBatch];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      a[2 * i] = __builtin_fmaf(
-          wt, __half2float(__ushort_as_half(uint16_t(p[i]))) * unit, a[2 * i]);
-      a[2 * i + 1] = __builtin_fmaf(
-          wt, __half2float(__ushort_as_half(uint16_t(p[i] >> 16))) * unit, a[2 * i + 1]);
+    for (int j = 0; j < kBatch; ++j) {
+      const int c = min(c0 + j, kk - 1);
+      const size_t r = size_t(n) * kk + c;
+      const u32x4* src = reinterpret_cast<const u32x4*>(y + r * d + d0);
+      if constexpr (PAST)
+        v[j] = __builtin_nontemporal_load(src);
+      else
+        v[j] = *src;
+      unit[j] = half_unit(yscale[r * (d / kMxGroup) + d0 / kMxGroup]);
+      wt[j] = c < k ? w[size_t(n) * k + c] : shared_logit ? psigmoid(shared_logit[n]) : 1.0f;
+      in[j] = c0 + j < kk && inv[r] >= 0;  // a dropped id's row holds anything
+    }
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      if (!in[j]) continue;
+      const uint32_t p[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        a[2 * i] = __builtin_fmaf(
+            wt[j], __half2float(__ushort_as_half(uint16_t(p[i]))) * unit[j], a[2 * i]);
+        a[2 * i + 1] = __builtin_fmaf(
+            wt[j], __half2float(__ushort_as_half(uint16_t(p[i] >> 16))) * unit[j], a[2 * i + 1]);
+      }
     }
   }
   uint32_t o[4];
@@ -829,6 +851,14 @@ __global__ __launch_bounds__(64 * kMaxWaves, 2) void mx_one_down_kernel(const Mx
   uint8_t* own = dyn + wave * batch * kOneItem;
   const uint32_t own_lds = __builtin_amdgcn_readfirstlane(
       uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)own)));
+  // lane c: column c's slot and weight, all looked up at once
+  int my_slot = -1;
+  float my_weight = 1.0f;
+  if (lane < a.kk) {
+    my_slot = a.slots[lane];
+    if constexpr (MIX)
+      my_weight = lane < a.k ? a.wts[lane] : a.shared_gate ? psigmoid(*a.shared_logit) : 1.0f;
+  }
   f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
   for (int t0 = wave; t0 < items; t0 += waves * batch) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -836,17 +866,18 @@ __global__ __launch_bounds__(64 * kMaxWaves, 2) void mx_one_down_kernel(const Mx
       const int t = t0 + b * waves;
       if (t >= items) break;
       const int c = first + t / stretches, j = t % stretches;
-      const int slot = __builtin_amdgcn_readfirstlane(a.slots[c]);
+      const int slot = __builtin_amdgcn_readlane(my_slot, c);
       if (slot < 0) continue;
       const uint8_t* base = a.slab + size_t(slot) * size_t(a.expert_bytes);
       one_fetch(own_lds + b * kOneItem, base + a.wd + size_t(f0) * row_bytes,
                 base + a.sd + size_t(f0) * groups, row_bytes, groups, j, lane);
     }
     {  // 16 lanes an item: a group of its column's h each
-      const int b = lane >> 4, t = t0 + b * waves;
-      if (b < batch && t < items) {
-        const int c = first + t / stretches, gi = 16 * (t % stretches) + (lane & 15);
-        if (gi < groups && a.slots[c] >= 0) {
+      const int b = lane >> 4, t = min(t0 + b * waves, items - 1);
+      const int c = first + t / stretches, gi = 16 * (t % stretches) + (lane & 15);
+      const int held = __shfl(my_slot, c, 64);  // of every lane: any may be asked
+      if (b < batch && t0 + b * waves < items) {
+        if (gi < groups && held >= 0) {
           const float4* src = reinterpret_cast<const float4*>(a.h + size_t(c) * a.inter + gi * kMxGroup);
           float v[32];
 #pragma unroll
@@ -869,13 +900,11 @@ __global__ __launch_bounds__(64 * kMaxWaves, 2) void mx_one_down_kernel(const Mx
       const int t = t0 + b * waves;
       if (t >= items) break;
       const int c = first + t / stretches, j = t % stretches;
-      if (__builtin_amdgcn_readfirstlane(a.slots[c]) < 0) continue;
+      if (__builtin_amdgcn_readlane(my_slot, c) < 0) continue;
       f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
       one_mma(acc, own + b * kOneItem, own + b * kOneItem + kOneFetch, min(16, groups - 16 * j),
                      lane);
-      float w = 1.0f;
-      if constexpr (MIX)
-        w = c < a.k ? a.wts[c] : a.shared_gate ? psigmoid(*a.shared_logit) : 1.0f;
+      const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(my_weight), c));
 #pragma unroll
       for (int i = 0; i < 4; ++i) sum[i] = MIX ? __builtin_fmaf(w, acc[i], sum[i]) : sum[i] + acc[i];
     }
@@ -931,6 +960,7 @@ template <bool DUAL, bool BLOCKS, bool HALF>
 __global__ __launch_bounds__(64 * kTileWaves, 2) void mx_tile_kernel(const MxArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kTileLds];
   __shared__ unsigned long long s_third;
+  __shared__ int32_t s_order[DUAL ? 1 : kTileRows];  // flat rows, for the stores
   constexpr int kCols = DUAL ? kTileCols / 2 : kTileCols;  // features a block
   const int fblocks = (a.features + kCols - 1) / kCols;
   // XCD x takes a contiguous range of the work, a tile's feature blocks side by
@@ -989,6 +1019,10 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void mx_tile_kernel(const MxArg
   const uint8_t* wscale = base + (second ? a.s1 : a.s0);
   const uint32_t w_off = uint32_t(lr) * uint32_t(a.cols / 2) + lq * 16;
   const uint32_t wscale_off = uint32_t(tile_row(4 * wave + q) + r) * uint32_t(groups);
+
+  if constexpr (!DUAL) {  // (the loop's barriers come before the reads)
+    if (int(threadIdx.x) < m) s_order[threadIdx.x] = a.order[p0 + threadIdx.x];
+  }
 
   Steps todo{0, steps};
   uint64_t thirds = 0;  // bit s: a row of the tile has a third piece in step s
@@ -1211,7 +1245,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void mx_tile_kernel(const MxArg
     for (int i = 0; i < 4; ++i) {
       const int row0 = 64 * rh + 16 * i;
       if (row0 >= m || f0 >= a.features) break;
-      const size_t own = row0 + r < m ? a.order[p0 + row0 + r] : 0;
+      const size_t own = row0 + r < m ? s_order[row0 + r] : 0;
       uint16_t o[32];
       if constexpr (HALF) {
 #pragma unroll
@@ -1241,9 +1275,14 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void mx_tile_kernel(const MxArg
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int row = 4 * j + (lane >> 4), c = f0 + 8 * (lane & 15);
-        const uint4 v = *reinterpret_cast<const uint4*>(ys + row * kPitch + (lane & 15) * 16);
-        if (row0 + row < m && c < a.features)
-          *reinterpret_cast<uint4*>(a.y + size_t(a.order[p0 + row0 + row]) * a.features + c) = v;
+        const u32x4 v = *reinterpret_cast<const u32x4*>(ys + row * kPitch + (lane & 15) * 16);
+        if (row0 + row < m && c < a.features) {
+          u32x4* to = reinterpret_cast<u32x4*>(a.y + size_t(s_order[row0 + row]) * a.features + c);
+          if (a.past_caches)
+            __builtin_nontemporal_store(v, to);
+          else
+            *to = v;
+        }
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
@@ -1366,6 +1405,7 @@ int mx_experts(const MxPlan& p, hipStream_t st) {
   a.pair = p.hpair, a.third = nullptr, a.ascale = p.hscale, a.asteps = nullptr;
   a.y = p.y;
   a.yscale = p.yscale;
+  a.past_caches = past_caches(int64_t(rows) * g->hidden);
   if (p.yscale)
     return large    ? launch_tile<false, true>(a, p.max_tiles, st)
            : stream ? launch_stream<false, true>(a, p.max_tiles, st)
@@ -1376,8 +1416,8 @@ int mx_experts(const MxPlan& p, hipStream_t st) {
 }
 
 // One token: two launches, no dispatch; out bf16 [hidden] combined (wts given), or
-// [kk, hidden].
-bool mx_one_covers(const pmoe_geom* g) { return mx_aligned(g); }
+// [kk, hidden].  Up to 64 columns: a lane looks one up.
+bool mx_one_covers(const pmoe_geom* g, int kk) { return kk <= 64 && mx_aligned(g); }
 
 int mx_one(const pmoe_geom* g, const uint8_t* slab, const int32_t* table, int n_experts,
            const uint16_t* x, const int32_t* ids, const float* wts, int k, int shared_slot,
@@ -1434,8 +1474,14 @@ int mx_combine(const uint16_t* y, const uint8_t* yscale, const float* w, const i
   const int blocks_row = (d / 8 + 255) / 256;
   PMOE_REQUIRE(int64_t(n) * blocks_row < (int64_t(1) << 31), "experts: too many rows for one call");
   ProfScope prof_scope(K_COMBINE, st);
-  mx_combine_kernel<<<unsigned(n) * blocks_row, 256, 0, st>>>(y, yscale, w, inv, shared_logit, k,
-                                                             kk, d, blocks_row, out);
+  const auto go = [&](auto kernel) {
+    kernel<<<unsigned(n) * blocks_row, 256, 0, st>>>(y, yscale, w, inv, shared_logit, k, kk, d,
+                                                     blocks_row, out);
+  };
+  if (past_caches(int64_t(n) * kk * d))
+    go(mx_combine_kernel<true>);
+  else
+    go(mx_combine_kernel<false>);
   PMOE_LAUNCH_CHECK("mx_combine_kernel");
   return PMOE_OK;
 }
