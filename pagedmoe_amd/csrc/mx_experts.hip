@@ -242,12 +242,20 @@ __global__ __launch_bounds__(1024) void mx_prepare_kernel(const MxSplit a, const
 // ---------------------------------------------------------------- memory to LDS
 
 // 16 bytes (4 bytes) a lane from base + voff to LDS [lds, lds + 1024) ([.., +
-// 256)), lane l at 16 l (4 l).  base and lds are the wave's.
+// 256)), lane l at 16 l (4 l).  base and lds are the wave's.  ONCE: nobody reads
+// them again (non-temporal).
+template <bool ONCE = false>
 __device__ __forceinline__ void dma16(uint32_t lds, uint32_t voff, const uint8_t* base) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-               :
-               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(uniform_ptr(base))
-               : "memory");
+  if constexpr (ONCE)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(uniform_ptr(base))
+                 : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(uniform_ptr(base))
+                 : "memory");
 }
 
 __device__ __forceinline__ void dma4(uint32_t lds, uint32_t voff, const uint8_t* base) {
@@ -433,7 +441,10 @@ constexpr int kStreamWave = kStreamRows * 128 + 2 * kStreamRows * 4;  // LDS of 
 // so that nothing waits for registers and the fetches are whole lines; two
 // blocks a CU keep 136 KB in flight.  (Loads into registers in the products' own
 // lane order, 16 bytes of 64 different rows an instruction, reached 3 TB/s.)
-template <bool DUAL, bool HALF>
+// ONCE: an expert has one tile on average, and its weights need no place in the
+// caches (us, gate/up + down, without / with it: 4096x1536 8 tokens 66 + 36 / 62 + 33,
+// 7168x2048 3 tokens 80 + 42 / 76 + 40).
+template <bool DUAL, bool HALF, bool ONCE>
 __global__ __launch_bounds__(64 * kMaxWaves, 4) void mx_stream_kernel(const MxArgs a) {
   constexpr int NF = 4;
   constexpr int kCols = DUAL ? kStreamRows / 2 : kStreamRows;  // features a block
@@ -521,7 +532,7 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void mx_stream_kernel(const MxAr
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         if (two || lp[i] < 4)
-          dma16(own_lds + f * 2048 + i * 1024, lrow * row_bytes + lp[i] * 16,
+          dma16<ONCE>(own_lds + f * 2048 + i * 1024, lrow * row_bytes + lp[i] * 16,
                 wbase[f] + size_t(8 * i) * row_bytes + j * 128);
     }
 #pragma unroll
@@ -602,7 +613,7 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void mx_stream_kernel(const MxAr
 }
 
 template <bool DUAL, bool HALF>
-int launch_stream(const MxArgs& a, int max_tiles, hipStream_t st) {
+int launch_stream(const MxArgs& a, int max_tiles, bool once, hipStream_t st) {
   constexpr int kCols = DUAL ? kStreamRows / 2 : kStreamRows;
   const int steps = (a.cols + kStreamStep - 1) / kStreamStep;
   const int rounds = (steps + kMaxWaves - 1) / kMaxWaves;
@@ -612,7 +623,10 @@ int launch_stream(const MxArgs& a, int max_tiles, hipStream_t st) {
   const size_t lds = std::max<size_t>(size_t(waves) * kStreamWave,
                                       size_t(waves) * 4096 + kFewRows * (kCols + 1) * 4);
   ProfScope prof_scope(DUAL ? K_MX_GATEUP : K_MX_DOWN, st);
-  mx_stream_kernel<DUAL, HALF><<<unsigned(blocks), 64 * waves, lds, st>>>(a);
+  if (once)
+    mx_stream_kernel<DUAL, HALF, true><<<unsigned(blocks), 64 * waves, lds, st>>>(a);
+  else
+    mx_stream_kernel<DUAL, HALF, false><<<unsigned(blocks), 64 * waves, lds, st>>>(a);
   PMOE_LAUNCH_CHECK("mx_stream_kernel");
   return PMOE_OK;
 }
@@ -1382,6 +1396,7 @@ int mx_experts(const MxPlan& p, hipStream_t st) {
   }
   const bool large = p.tile_rows == kTileRows;
   const bool stream = mx_aligned(g);
+  const bool once = rows <= int64_t(kFewRows) * p.n_experts;
   MxArgs a{};
   a.slab = p.slab;
   a.expert_bytes = g->expert_bytes;
@@ -1396,7 +1411,7 @@ int mx_experts(const MxPlan& p, hipStream_t st) {
   a.pair = p.xpair, a.third = p.xthird, a.ascale = p.xscale, a.asteps = p.xsteps;
   a.hpair = p.hpair, a.hscale = p.hscale;
   if (int rc = large    ? launch_tile<true, false>(a, p.max_tiles, st)
-               : stream ? launch_stream<true, false>(a, p.max_tiles, st)
+               : stream ? launch_stream<true, false>(a, p.max_tiles, once, st)
                         : launch_small<true, false>(a, p.max_tiles, st))
     return rc;
   a.w0 = g->off[PMOE_DOWN_W], a.s0 = g->off[PMOE_DOWN_S];
@@ -1408,10 +1423,10 @@ int mx_experts(const MxPlan& p, hipStream_t st) {
   a.past_caches = past_caches(int64_t(rows) * g->hidden);
   if (p.yscale)
     return large    ? launch_tile<false, true>(a, p.max_tiles, st)
-           : stream ? launch_stream<false, true>(a, p.max_tiles, st)
+           : stream ? launch_stream<false, true>(a, p.max_tiles, once, st)
                     : launch_small<false, true>(a, p.max_tiles, st);
   return large    ? launch_tile<false, false>(a, p.max_tiles, st)
-         : stream ? launch_stream<false, false>(a, p.max_tiles, st)
+         : stream ? launch_stream<false, false>(a, p.max_tiles, once, st)
                   : launch_small<false, false>(a, p.max_tiles, st);
 }
 
