@@ -111,6 +111,18 @@ def test_format_long_arrays():
     assert np.array_equal(back[rows].double().cpu().numpy(), M.dequant(c, sc))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_format_past_the_caches(dtype):
+    """Results of more than 64 MiB: the same values as in parts below that."""
+    g = torch.Generator(device=DEV).manual_seed(1)
+    w = torch.randn(4100, 8192, device=DEV, generator=g).to(dtype)
+    q, s = K.mx4_quantize(w)
+    whole = K.mx4_dequant(q, s, dtype)
+    for a in range(0, 4100, 1025):
+        part = K.mx4_dequant(q[a:a + 1025].contiguous(), s[a:a + 1025].contiguous(), dtype)
+        assert torch.equal(whole[a:a + 1025], part)
+
+
 # ---------------------------------------------------------------- experts
 
 class Layer:
@@ -482,6 +494,92 @@ def test_checkpoint_to_output(tmp_path):
                     for q in ("gate_proj", "up_proj", "down_proj")]
             ref, b = M.ffn(x[n:n + 1].double().cpu().numpy(), *mats)
             assert (np.abs(y[n, c] - ref[0]) <= b[0] * (1 + 2.0 ** -8) + np.abs(ref[0]) * 2.0 ** -8).all()
+
+
+@pytest.mark.parametrize("n,k", [(1, 70), (3, 70), (1, 17)])
+def test_many_columns(n, k):
+    """More columns than a wave has lanes (one token's two launches stop there)."""
+    rng = np.random.default_rng(k)
+    L = Layer(256, 128, 80, 1)
+    x = tokens(rng, n, 256)
+    inds = np.stack([rng.permutation(80)[:k] for _ in range(n)]).astype(np.int32)
+    inds[0, 3] = -1
+    w = rng.random((n, k)).astype(np.float32)
+    out = K.moe_experts(L.g, L.slab.buf, L.table, 80, x, torch.from_numpy(inds).to(DEV),
+                        torch.from_numpy(w).to(DEV), L.shared_slot, None)
+    ref, b = combined(L, x.double().cpu().numpy(), inds, w.astype(np.float64))
+    check(out, ref, b)
+    y = K.switch_glu(L.g, L.slab.buf, L.table, 80, x, torch.from_numpy(inds).to(DEV))
+    ref, b = L.seam(x.double().cpu().numpy(), inds)
+    check(y, ref, b)
+
+
+@pytest.mark.parametrize("n", [1, 5])
+def test_overflow_is_nan(n):
+    """An intermediate beyond fp32 makes its row NaN, not a plausible number."""
+    rng = np.random.default_rng(0)
+    L = Layer(256, 128, 2)
+    x = tokens(rng, n, 256)
+    x[0] = (x[0].float() * 2.0 ** 70).to(torch.bfloat16)
+    inds = torch.zeros(n, 1, dtype=torch.int32, device=DEV)
+    y = K.switch_glu(L.g, L.slab.buf, L.table, 2, x, inds)
+    assert torch.isnan(y[0]).all() and torch.isfinite(y[1:]).all()
+    out = K.moe_experts(L.g, L.slab.buf, L.table, 2, x, inds, torch.ones(n, 1, device=DEV))
+    assert torch.isnan(out[0]).all() and torch.isfinite(out[1:]).all()
+
+
+@pytest.mark.parametrize("n", [1, 6])
+def test_block_without_allocation(n):
+    """pmoe_moe_block_noalloc gives pmoe_moe_block's bits, captured too."""
+    import ctypes
+    rng = np.random.default_rng(n)
+    L = Layer(512, 128, 16, 1)
+    x = tokens(rng, n, 512)
+    gate_w = bf16(rng.standard_normal((16, 512)) * 0.05)
+    rc = K.route_cfg("softmax", 16, 4)
+    ref, ri, rw = K.moe_block(L.g, rc, L.slab.buf, L.table, gate_w, x, shared_slot=16)
+    out, inds, w = torch.empty_like(ref), torch.empty_like(ri), torch.empty_like(rw)
+
+    def go():
+        _lib.check(_lib.lib().pmoe_moe_block_noalloc(
+            ctypes.byref(L.g), ctypes.byref(rc), L.slab.buf.data_ptr(), L.table.data_ptr(),
+            gate_w.data_ptr(), None, None, x.data_ptr(), n, 16, None, out.data_ptr(),
+            inds.data_ptr(), w.data_ptr(), K._stream()))
+    go()
+    assert torch.equal(out, ref) and torch.equal(inds, ri) and torch.equal(w, rw)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        go()
+    for _ in range(3):
+        x.copy_(tokens(rng, n, 512))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, K.moe_block(L.g, rc, L.slab.buf, L.table, gate_w, x,
+                                            shared_slot=16)[0])
+
+
+@pytest.mark.parametrize("n", [140, 1500])
+def test_large_calls_gate_and_zero_rows(n):
+    """Calls whose dispatch takes several launches: the gated shared expert, and the
+    seam's zero rows of dropped ids."""
+    rng = np.random.default_rng(n)
+    L = Layer(256, 128, 6, 1)
+    x = tokens(rng, n, 256)
+    inds = rng.integers(-1, 7, (n, 8)).astype(np.int32)
+    w = rng.random((n, 8)).astype(np.float32)
+    gate = bf16(rng.standard_normal((1, 256)) * 0.05)
+    t = torch.from_numpy(inds).to(DEV)
+    out = K.moe_experts(L.g, L.slab.buf, L.table, 6, x, t, torch.from_numpy(w).to(DEV), 6, gate)
+    xd = x.double().cpu().numpy()
+    ref, b = combined(L, xd, inds, w.astype(np.float64), gate.double().cpu().numpy())
+    check(out, ref, b)
+    y = K.switch_glu(L.g, L.slab.buf, L.table, 6, x, t)
+    ref, b = L.seam(xd, inds)
+    check(y, ref, b)
+    gone = torch.from_numpy((inds < 0) | (inds >= 6))
+    assert (y.cpu()[gone].view(torch.int16) == 0).all()
 
 
 def test_empty_call():

@@ -165,6 +165,23 @@ def test_rows_off_16_bytes_give_the_same_rows():
         check(b)
 
 
+@pytest.mark.parametrize("stream", [torch.bfloat16, torch.float32])
+def test_past_the_caches(stream):
+    """Results of more than 64 MiB, in place too: the rows that shorter calls give."""
+    a = make(8500, 4096, 0, stream, torch.bfloat16, "element", True, True, 0, 2)
+    out, h = run(a)
+    nh = K.block_norm(a["residual"], a["next_weight"])
+    for r0 in (0, 4000, 8400):
+        part = {k: v[r0:r0 + 100].contiguous() if torch.is_tensor(v) and v.dim() == 2 else v
+                for k, v in a.items()}
+        o, hh = run(part)
+        assert torch.equal(out[r0:r0 + 100], o) and torch.equal(h[r0:r0 + 100], hh)
+        assert torch.equal(nh[r0:r0 + 100], K.block_norm(part["residual"], a["next_weight"]))
+    res = a["residual"]
+    o, hh = run(a, out=res)
+    assert o is res and torch.equal(o, out) and torch.equal(hh, h)
+
+
 def test_special_rows():
     """A zero row stays zero (eps keeps the norm finite); an infinity or NaN
     makes its own row's h NaN and no other row's."""
