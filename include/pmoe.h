@@ -328,7 +328,8 @@ typedef struct {
 
 /* h = w * x / sqrt(mean(x^2) + eps) over each row of x [n, hidden] (fp32 or
  * bf16; weight [hidden] fp32 or bf16; 1 + weight with unit_offset), bf16 out.
- * hidden: 1..16384.  The sum of a row's squares must stay inside fp32. */
+ * hidden: 1..16384; n: up to 2^23.  The sum of a row's squares must stay inside
+ * fp32 (and above its smallest numbers where eps is no larger). */
 int pmoe_block_norm(const void* x, int x_dtype, const void* weight, int weight_dtype, int n,
                     int hidden, float eps, int unit_offset, void* h, void* stream);
 
@@ -341,7 +342,8 @@ int pmoe_block_norm(const void* x, int x_dtype, const void* weight, int weight_d
  *          (NULL: no h; h bf16 [n, hidden])
  *   gate   of gate_kind (NULL: none)
  * residual and out are [n, hidden] of stream_dtype; out may be residual.  All in
- * fp32, each result rounded once (h from out before its rounding). */
+ * fp32, each result rounded once (h from out before its rounding).  Sizes as in
+ * pmoe_block_norm. */
 int pmoe_block_join(const pmoe_join* j, const void* residual, const void* y, const float* weights,
                     const void* shared_y, const float* shared_logit, const void* post_weight,
                     const void* gate, const void* next_weight, int n, int k, int hidden, void* out,

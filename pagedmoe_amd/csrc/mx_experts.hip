@@ -421,7 +421,6 @@ int launch_small(const MxArgs& a, int max_tiles, hipStream_t st) {
   const int rounds = (steps + kMaxWaves - 1) / kMaxWaves;
   const int waves = (steps + rounds - 1) / rounds;
   const int64_t blocks = int64_t(max_tiles) * (a.features / kSmallCols);
-  PMOE_REQUIRE(blocks < (int64_t(1) << 31) / 1, "experts: too many tiles for one call");
   ProfScope prof_scope(DUAL ? K_MX_GATEUP : K_MX_DOWN, st);
   mx_small_kernel<DUAL, HALF><<<unsigned(blocks), 64 * waves, 0, st>>>(a);
   PMOE_LAUNCH_CHECK("mx_small_kernel");
@@ -619,7 +618,6 @@ int launch_stream(const MxArgs& a, int max_tiles, bool once, hipStream_t st) {
   const int rounds = (steps + kMaxWaves - 1) / kMaxWaves;
   const int waves = (steps + rounds - 1) / rounds;
   const int64_t blocks = int64_t(max_tiles) * ((a.features + kCols - 1) / kCols);
-  PMOE_REQUIRE(blocks < (int64_t(1) << 31), "experts: too many tiles for one call");
   const size_t lds = std::max<size_t>(size_t(waves) * kStreamWave,
                                       size_t(waves) * 4096 + kFewRows * (kCols + 1) * 4);
   ProfScope prof_scope(DUAL ? K_MX_GATEUP : K_MX_DOWN, st);
@@ -1307,7 +1305,6 @@ template <bool DUAL, bool HALF>
 int launch_tile(const MxArgs& a, int max_tiles, hipStream_t st) {
   constexpr int kCols = DUAL ? kTileCols / 2 : kTileCols;
   const int64_t blocks = (int64_t(max_tiles) * ((a.features + kCols - 1) / kCols) + 7) / 8 * 8;
-  PMOE_REQUIRE(blocks < (int64_t(1) << 31), "experts: too many tiles for one call");
   ProfScope prof_scope(DUAL ? K_MX_GATEUP : K_MX_DOWN, st);
   const int64_t scales = DUAL ? a.s0 | a.s1 : a.s0;
   if (a.cols % kStep == 0 && (scales | a.expert_bytes) % 16 == 0)
@@ -1366,7 +1363,19 @@ int mx_experts(const MxPlan& p, hipStream_t st) {
   const pmoe_geom* g = p.geom;
   const bool shared = p.kk > p.k;
   const int n_ids = p.n_experts + (shared ? 1 : 0), rows = p.n * p.kk;
+  const bool large = p.tile_rows == kTileRows;
+  const bool stream = mx_aligned(g);
   PMOE_REQUIRE(n_ids <= kMaxExperts, "dispatch: experts must be 1..1024");
+  {  // a launch holds less than 2^32 threads: the split's, the combine's, the products'
+    const int up_cols = large ? kTileCols / 2 : kSmallCols;
+    const int down_cols = large ? kTileCols : stream ? kStreamRows : kSmallCols;
+    const int64_t blocks = std::max((g->inter + up_cols - 1) / up_cols,
+                                    (g->hidden + down_cols - 1) / down_cols);
+    const int64_t row_blocks = (g->hidden + 2047) / 2048;
+    PMOE_REQUIRE(p.n * row_blocks < int64_t(1) << 24 &&
+                     p.max_tiles * blocks <= (int64_t(1) << 23) - 8,
+                 "experts: too many rows for one call");
+  }
   MxSplit sp{};
   sp.x = p.x;
   sp.n = p.n, sp.groups = g->hidden / kMxGroup, sp.steps = mx_steps(g->hidden);
@@ -1394,8 +1403,6 @@ int mx_experts(const MxPlan& p, hipStream_t st) {
     mx_split_kernel<<<p.n, 256, 0, st>>>(sp);
     PMOE_LAUNCH_CHECK("mx_split_kernel");
   }
-  const bool large = p.tile_rows == kTileRows;
-  const bool stream = mx_aligned(g);
   const bool once = rows <= int64_t(kFewRows) * p.n_experts;
   MxArgs a{};
   a.slab = p.slab;
@@ -1487,7 +1494,6 @@ int mx_combine(const uint16_t* y, const uint8_t* yscale, const float* w, const i
                const float* shared_logit, int n, int k, int kk, int d, uint16_t* out,
                hipStream_t st) {
   const int blocks_row = (d / 8 + 255) / 256;
-  PMOE_REQUIRE(int64_t(n) * blocks_row < (int64_t(1) << 31), "experts: too many rows for one call");
   ProfScope prof_scope(K_COMBINE, st);
   const auto go = [&](auto kernel) {
     kernel<<<unsigned(n) * blocks_row, 256, 0, st>>>(y, yscale, w, inv, shared_logit, k, kk, d,

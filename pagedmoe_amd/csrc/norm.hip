@@ -28,6 +28,7 @@ namespace {
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kMaxHidden = 16384;  // 256 threads with 64 elements each
+constexpr int kMaxRows = 1 << 23;  // a launch holds less than 2^32 threads
 
 struct JoinArgs {
   const void* residual;
@@ -371,6 +372,7 @@ extern "C" int pmoe_block_norm(const void* x, int x_dtype, const void* weight, i
                "block_norm: arrays are fp32 or bf16");
   PMOE_REQUIRE(n >= 0 && hidden > 0 && hidden <= kMaxHidden,
                "block_norm: hidden must be 1..16384");
+  PMOE_REQUIRE(n <= kMaxRows, "block_norm: more than 2^23 rows");
   PMOE_REQUIRE(eps >= 0.0f, "block_norm: eps must not be negative");
   if (n == 0) return PMOE_OK;
   hipStream_t st = static_cast<hipStream_t>(stream);
@@ -405,6 +407,7 @@ extern "C" int pmoe_block_join(const pmoe_join* j, const void* residual, const v
                "block_join: arrays are fp32 or bf16");
   PMOE_REQUIRE(n >= 0 && k > 0 && hidden > 0 && hidden <= kMaxHidden,
                "block_join: bad shape (hidden must be 1..16384)");
+  PMOE_REQUIRE(n <= kMaxRows, "block_join: more than 2^23 rows");
   PMOE_REQUIRE(weights || k == 1, "block_join: several slots need weights");
   PMOE_REQUIRE(!shared_logit || shared_y, "block_join: shared_logit without shared_y");
   PMOE_REQUIRE((j->gate_kind == PMOE_GATE_NONE) == (gate == nullptr) &&

@@ -510,7 +510,8 @@ class MoELayer(nn.Module):
     def forward(self, x: torch.Tensor, gate: torch.Tensor | None = None,
                 h: torch.Tensor | None = None, next_weight: torch.Tensor | None = None):
         """x [..., D] (a bf16 or fp32 residual stream) -> out like x.  ``gate``
-        replaces the layer's for this call.  With ``next_weight`` [D] also the
+        replaces the layer's for this call (per token or element also in x's
+        own leading dims).  With ``next_weight`` [D] also the
         next norm of out, in the same launch: (out, h [..., D] bf16); that ``h``
         is what the next layer takes here in place of its own first norm."""
         d = x.shape[-1]
@@ -519,6 +520,8 @@ class MoELayer(nn.Module):
             h = K.block_norm(x2, self.pre_weight, self.eps, self.unit_offset)
         y, w, shared_y, shared_logit = self.block.mixture(h.reshape(-1, d))
         gate = self.gate if gate is None else gate
+        if gate is not None and gate.dim() > 2:  # [.., 1] or [.., D] beside x
+            gate = gate.reshape(-1, gate.shape[-1])
         out, nh = K.block_join(
             x2, y, w, shared_y=shared_y, shared_logit=shared_logit, post_weight=self.post_weight,
             gate=gate, gate_sigmoid=self.gate_sigmoid, residual_scale=self.residual_scale,

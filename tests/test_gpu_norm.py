@@ -297,3 +297,21 @@ def test_layers(group, paged):
         assert (b.double() - r).norm() <= 2.0 ** -7 * r.norm()
     y = layers[0].block(x.to(torch.bfloat16).reshape(2, 50, hidden))
     assert y.shape == (2, 50, hidden)
+
+
+def test_layer_gates_beside_leading_dims():
+    """A gate given in x's own leading dims is the one of the flat rows."""
+    hidden, inter, experts = 256, 128, 8
+    g = gen(4)
+    rn = lambda *s: torch.randn(*s, device=DEV, generator=g)  # noqa: E731
+    glu = S.QuantizedSwitchGLU(hidden, inter, experts, 4, 32)
+    for e in range(experts):
+        glu.quantize_expert(e, rn(inter, hidden) * 0.05, rn(inter, hidden) * 0.05,
+                            rn(hidden, inter) * 0.05)
+    layer = S.MoELayer(S.SoftmaxMoEBlock(rn(experts, hidden) * 0.1, glu, 2), torch.ones(hidden, device=DEV),
+                       gate_sigmoid=True)
+    x = rn(2, 5, hidden)
+    for gate in (rn(2, 5, 1), rn(2, 5, hidden)):
+        out = layer(x, gate=gate)
+        flat = layer(x.reshape(10, hidden), gate=gate.reshape(10, -1))
+        assert out.shape == x.shape and torch.equal(out.reshape(10, hidden), flat)

@@ -129,6 +129,21 @@ def test_expert_entries_refuse_a_small_workspace():
     assert L.pmoe_switch_glu(ctypes.byref(g), D, D, 8, D, D, 5, 2, D, D, need - 1, None) == -5
 
 
+@pytest.mark.parametrize("hidden,inter,n,k", [
+    (1024, 512, 1 << 24, 1),     # the split's blocks
+    (8192, 512, 1 << 22, 2),     # the combine's
+    (1056, 480, 3 << 20, 4),     # small tiles
+    (8192, 8192, 700000, 8)])    # large ones
+def test_expert_entries_refuse_more_rows_than_a_launch_holds(hidden, inter, n, k):
+    """On the host, before the first launch; the dummy pointers are never read."""
+    L = _lib.lib()
+    p = ctypes.byref(_lib.geom(hidden, inter, 4, 32))
+    assert L.pmoe_switch_glu(p, D, D, 8, D, D, n, k, D, D, 1 << 60, None) == -1
+    assert b"too many rows" in L.pmoe_last_error()
+    assert L.pmoe_moe_experts(p, D, D, 8, D, D, D, n, k, -1, None, D, D, 1 << 60, None) == -1
+    assert b"too many rows" in L.pmoe_last_error()
+
+
 # ---------------------------------------------------------------- the oracle
 
 def test_oracle_rounds_to_nearest_with_ties_to_even():
