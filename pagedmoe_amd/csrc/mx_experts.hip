@@ -31,6 +31,7 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kFp4 = 4, kFp6 = 2;  // operand formats of the scaled MFMA
+constexpr int kStretch = 512;      // values of a row whose scales are 16 bytes
 
 __device__ __forceinline__ const uint8_t* uniform_ptr(const uint8_t* p) {
   const uint64_t v = reinterpret_cast<uint64_t>(p);
@@ -274,168 +275,18 @@ __device__ __forceinline__ int swizzle4(int r) { return -(r >> 2) & 3; }
 __device__ __forceinline__ int swizzle8(int r) { return (r >> 1 & 4) | (r & 2); }
 __device__ __forceinline__ int swizzle16(int r) { return (r & 3) << 1 | (r & 8); }
 
-// ---------------------------------------------------------------- small tiles
-
-constexpr int kFewRows = 16;     // activation rows a tile
-constexpr int kSmallCols = 32;   // features a block (one group of the next product)
-constexpr int kStep = 512;       // reduction that a wave takes at a time
-constexpr int kMaxWaves = 8;
-
-// One tile of at most 16 rows of an expert times 32 features (DUAL: 32 gate
-// and the same 32 up features), for reductions of any number of groups.  The
-// waves share the reduction: wave w takes steps w, w + waves, ... of 512, and
-// the partial sums meet in LDS.
-template <bool DUAL, bool HALF>
-__global__ __launch_bounds__(64 * kMaxWaves) void mx_small_kernel(const MxArgs a) {
-  constexpr int NF = DUAL ? 4 : 2;  // 16-feature tiles: gate, gate, up, up
-  __shared__ float s_red[kMaxWaves][NF * 4][64];
-  __shared__ float s_h[kFewRows][kSmallCols + 1];
-  const int fblocks = a.features / kSmallCols;
-  const int t = blockIdx.x / fblocks;
-  const int fb = blockIdx.x - t * fblocks;
-  if (t >= *a.n_tiles) return;
-  const int4 tile = a.tiles[t];  // {slot, first row, rows of the expert, offset}
-  const int m = min(kFewRows, tile.z - tile.y);
-  const int p0 = tile.w + tile.y;
-  const int waves = blockDim.x >> 6;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (tile.x < 0) {  // not resident: exact zero rows
-    if constexpr (!DUAL) {
-      for (int i = threadIdx.x; i < m * kSmallCols; i += blockDim.x) {
-        const size_t flat = a.order[p0 + i / kSmallCols];
-        a.y[flat * a.features + fb * kSmallCols + i % kSmallCols] = 0;
-        if (HALF && i % kSmallCols == 0) a.yscale[flat * fblocks + fb] = 1;
-      }
-    }
-    return;
-  }
-  const int r = lane & 15, q = lane >> 4;
-  const int pos = p0 + (r < m ? r : 0);
-  const size_t arow = DUAL ? size_t(a.order[pos] / a.kk) : size_t(pos);
-  const int groups = a.cols / kMxGroup;
-  const uint8_t* base = a.slab + size_t(tile.x) * size_t(a.expert_bytes);
-  const uint8_t* wrow[NF];
-  const uint8_t* srow[NF];
-#pragma unroll
-  for (int f = 0; f < NF; ++f) {
-    const size_t row = size_t(fb) * kSmallCols + (f & 1) * 16 + r;
-    wrow[f] = base + (f < 2 ? a.w0 : a.w1) + row * size_t(a.cols / 2);
-    srow[f] = base + (f < 2 ? a.s0 : a.s1) + row * size_t(groups);
-  }
-  const size_t asteps = arow * mx_steps(a.cols);
-  const uint8_t* pair = a.pair + asteps * kMxStepPair;
-  const uint8_t* third = DUAL ? a.third + asteps * kMxStepThird : nullptr;
-  const uint8_t* ascale = a.ascale + arow * mx_scale_row(a.cols);
-  f32x4 acc[NF];
-#pragma unroll
-  for (int f = 0; f < NF; ++f) acc[f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  const int steps = (groups + 15) / 16;
-  for (int j = wave; j < steps; j += waves) {
-    uint4 w[NF][4];
-    int sw[NF][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int g = 16 * j + 4 * i + q;
-      const bool in = g < groups;
-#pragma unroll
-      for (int f = 0; f < NF; ++f) {
-        w[f][i] = in ? *reinterpret_cast<const uint4*>(wrow[f] + size_t(g) * 16)
-                     : make_uint4(0, 0, 0, 0);
-        sw[f][i] = in ? srow[f][g] : 127;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int g = 16 * j + 4 * i + q;
-      const bool in = g < groups;
-      const int gc = in ? g : 0;
-      const uint4* src =
-          reinterpret_cast<const uint4*>(pair + (gc >> 2) * kMxStepPair + (gc & 3) * 16);
-      const uint4 c0 = src[0], c1 = src[kMxChunk / 16], c2 = src[2 * kMxChunk / 16];
-      const int sa = in ? ascale[mx_scale_at(gc)] : 127;
-      const uint32_t b0[6] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y};
-      const uint32_t b1[6] = {c1.z, c1.w, c2.x, c2.y, c2.z, c2.w};
-#pragma unroll
-      for (int f = 0; f < NF; ++f) mx_mma(acc[f], w[f][i], sw[f][i], b0, sa);
-#pragma unroll
-      for (int f = 0; f < NF; ++f)
-        mx_mma(acc[f], w[f][i], sw[f][i], b1, sa - (DUAL ? kMxTokenShift : kMxInterShift));
-      if constexpr (DUAL) {
-        const uint4 d = *reinterpret_cast<const uint4*>(third + (gc >> 2) * kMxStepThird +
-                                                        (gc & 3) * 16);
-#pragma unroll
-        for (int f = 0; f < NF; ++f) mx_mma_third(acc[f], w[f][i], sw[f][i], d, sa);
-      }
-    }
-  }
-#pragma unroll
-  for (int f = 0; f < NF; ++f)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s_red[wave][4 * f + i][lane] = acc[f][i];
-  __syncthreads();
-  // feature c of row s_r: accumulator c % 4 of lane 16 (c % 16 / 4) + row
-  for (int i = threadIdx.x; i < kFewRows * kSmallCols; i += blockDim.x) {
-    const int row = i / kSmallCols, c = i % kSmallCols;
-    if (row >= m) break;  // whole halves of a wave
-    const int src = (c & 15) / 4 * 16 + row;
-    float v = 0.0f, u = 0.0f;
-    for (int k = 0; k < waves; ++k) {
-      v += s_red[k][4 * (c >> 4) + (c & 3)][src];
-      if constexpr (DUAL) u += s_red[k][4 * (2 + (c >> 4)) + (c & 3)][src];
-    }
-    if constexpr (DUAL)
-      s_h[row][c] = silu_fast(v) * u;
-    else {
-      const size_t flat = a.order[p0 + row];
-      uint16_t* y = a.y + flat * a.features + fb * kSmallCols + c;
-      if constexpr (HALF) {
-        const int sc = half_scale(half_wave_max(__float_as_uint(v) & 0x7fffffffu));
-        *y = half_of(v, sc);
-        if (c == 0) a.yscale[flat * fblocks + fb] = uint8_t(sc);
-      } else {
-        *y = f2bf(v);
-      }
-    }
-  }
-  if constexpr (DUAL) {
-    __syncthreads();
-    if (int(threadIdx.x) < m) {
-      float v[32];
-#pragma unroll
-      for (int c = 0; c < 32; ++c) v[c] = s_h[threadIdx.x][c];
-      int s;
-      u32x6 h0, h1;
-      uint4 none;
-      mx_split<false>(v, s, h0, h1, none);
-      const size_t row = size_t(p0 + threadIdx.x) * mx_steps(a.features);
-      mx_store_pair(a.hpair + row * kMxStepPair, fb, h0, h1);
-      a.hscale[size_t(p0 + threadIdx.x) * mx_scale_row(a.features) + mx_scale_at(fb)] = uint8_t(s);
-    }
-  }
-}
-
-template <bool DUAL, bool HALF>
-int launch_small(const MxArgs& a, int max_tiles, hipStream_t st) {
-  const int steps = (a.cols + kStep - 1) / kStep;
-  const int rounds = (steps + kMaxWaves - 1) / kMaxWaves;
-  const int waves = (steps + rounds - 1) / rounds;
-  const int64_t blocks = int64_t(max_tiles) * (a.features / kSmallCols);
-  ProfScope prof_scope(DUAL ? K_MX_GATEUP : K_MX_DOWN, st);
-  mx_small_kernel<DUAL, HALF><<<unsigned(blocks), 64 * waves, 0, st>>>(a);
-  PMOE_LAUNCH_CHECK("mx_small_kernel");
-  return PMOE_OK;
-}
-
 // ---------------------------------------------------------------- streamed tiles
 
+constexpr int kFewRows = 16;                       // activation rows a tile
+constexpr int kMaxWaves = 8;
 constexpr int kStreamStep = 256;                   // reduction that a wave takes at a time
 constexpr int kStreamRows = 64;                    // weight rows a block
 constexpr int kStreamWave = kStreamRows * 128 + 2 * kStreamRows * 4;  // LDS of a wave
 
-// As mx_small_kernel, for reductions of whole steps of 128: one tile of at most
-// 16 rows times 64 weight rows (DUAL: 32 gate and the same 32 up features; 64
-// features otherwise).  Bound by the weights' stream: a wave's 64 rows x 128
+// One tile of at most 16 rows of an expert times 64 weight rows (DUAL: 32 gate and
+// the same 32 up features; 64 features otherwise).  The waves share the reduction:
+// wave w takes steps w, w + waves, ... of 256, and the partial sums meet in LDS.
+// Bound by the weights' stream: a wave's 64 rows x 128
 // bytes go straight into its own LDS, 8 lanes side by side on a row's 128 bytes,
 // so that nothing waits for registers and the fetches are whole lines; two
 // blocks a CU keep 136 KB in flight.  (Loads into registers in the products' own
@@ -443,7 +294,10 @@ constexpr int kStreamWave = kStreamRows * 128 + 2 * kStreamRows * 4;  // LDS of 
 // ONCE: an expert has one tile on average, and its weights need no place in the
 // caches (us, gate/up + down, without / with it: 4096x1536 8 tokens 66 + 36 / 62 + 33,
 // 7168x2048 3 tokens 80 + 42 / 76 + 40).
-template <bool DUAL, bool HALF, bool ONCE>
+// WHOLE: the reduction is whole steps of 128, and its scales lie on 4 bytes, so that
+// they come the weights' way; otherwise through registers, and groups past the
+// row's end count as zeros.
+template <bool DUAL, bool HALF, bool ONCE, bool WHOLE>
 __global__ __launch_bounds__(64 * kMaxWaves, 4) void mx_stream_kernel(const MxArgs a) {
   constexpr int NF = 4;
   constexpr int kCols = DUAL ? kStreamRows / 2 : kStreamRows;  // features a block
@@ -472,7 +326,8 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void mx_stream_kernel(const MxAr
     return;
   }
   const int r = lane & 15, q = lane >> 4;
-  const int groups = a.cols / kMxGroup, steps = groups / kMxStepGroups;
+  const int groups = a.cols / kMxGroup;
+  const int steps = (groups + kMxStepGroups - 1) / kMxStepGroups;
   const uint8_t* base = a.slab + size_t(tile.x) * size_t(a.expert_bytes);
   const uint32_t row_bytes = a.cols / 2;
   // weight tile f: 16 features from f16 of projection f / 2 (DUAL); tiles past the
@@ -502,6 +357,9 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void mx_stream_kernel(const MxAr
   for (int f = 0; f < NF; ++f) acc[f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   for (int j = wave; 2 * j < steps; j += waves) {
     const bool two = 2 * j + 1 < steps;  // the step's second half is there
+    const auto group_in = [&](int i) {   // the lane's group of half i is there
+      return WHOLE ? i == 0 || two : 8 * j + 4 * i + q < groups;
+    };
     // this step's activations (rows that are not there: zeros)
     uint4 c[2][3], d[2];
     uint32_t sa4 = 0;
@@ -514,7 +372,7 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void mx_stream_kernel(const MxAr
     if (live) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        if (i == 0 || two) {
+        if (group_in(i)) {
           const uint8_t* src = pair + (2 * j + i) * kMxStepPair;
 #pragma unroll
           for (int k = 0; k < 3; ++k) c[i][k] = *reinterpret_cast<const uint4*>(src + k * kMxChunk);
@@ -524,26 +382,46 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void mx_stream_kernel(const MxAr
       }
       sa4 = *reinterpret_cast<const uint32_t*>(ascale + (j >> 1) * kMxScaleBlock);
     }
+    uint32_t sword[2] = {0x7f7f7f7f, 0x7f7f7f7f};
+    if constexpr (!WHOLE) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int g = 8 * j + 4 * i;
+        if (g + 4 <= groups) {
+          __builtin_memcpy(&sword[i], sbase + g, 4);
+        } else {
+#pragma unroll
+          for (int b = 0; b < 3; ++b)
+            if (g + b < groups)
+              sword[i] = (sword[i] & ~(0xffu << 8 * b)) | uint32_t(sbase[g + b]) << 8 * b;
+        }
+      }
+    }
     // the LDS reads of the step before are done
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
     for (int f = 0; f < NF; ++f) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        if (two || lp[i] < 4)
+        if (WHOLE ? two || lp[i] < 4 : 8 * j + lp[i] < groups)
           dma16<ONCE>(own_lds + f * 2048 + i * 1024, lrow * row_bytes + lp[i] * 16,
-                wbase[f] + size_t(8 * i) * row_bytes + j * 128);
+                      wbase[f] + size_t(8 * i) * row_bytes + j * 128);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      if (i == 0 || two)
+      if (WHOLE && (i == 0 || two))
         dma4(own_lds + NF * 2048 + i * 256, uint32_t(sbase - base) + (2 * j + i) * 4, base);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if constexpr (!WHOLE)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        *reinterpret_cast<uint32_t*>(own + NF * 2048 + i * 256 + lane * 4) = sword[i];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if (i && !two) break;
       const int at = (r * 8 + ((4 * i + q) ^ swizzle8(r))) * 16;
-      const int sa = int(sa4 >> (8 * (2 * (j & 1) + i)));
+      // (an absent group's scale byte was never written)
+      const int sa = group_in(i) ? int(sa4 >> (8 * (2 * (j & 1) + i))) : 127;
       uint4 w[NF];
       int sw[NF];
 #pragma unroll
@@ -612,7 +490,7 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void mx_stream_kernel(const MxAr
 }
 
 template <bool DUAL, bool HALF>
-int launch_stream(const MxArgs& a, int max_tiles, bool once, hipStream_t st) {
+int launch_stream(const MxArgs& a, int max_tiles, bool once, bool whole, hipStream_t st) {
   constexpr int kCols = DUAL ? kStreamRows / 2 : kStreamRows;
   const int steps = (a.cols + kStreamStep - 1) / kStreamStep;
   const int rounds = (steps + kMaxWaves - 1) / kMaxWaves;
@@ -621,10 +499,13 @@ int launch_stream(const MxArgs& a, int max_tiles, bool once, hipStream_t st) {
   const size_t lds = std::max<size_t>(size_t(waves) * kStreamWave,
                                       size_t(waves) * 4096 + kFewRows * (kCols + 1) * 4);
   ProfScope prof_scope(DUAL ? K_MX_GATEUP : K_MX_DOWN, st);
-  if (once)
-    mx_stream_kernel<DUAL, HALF, true><<<unsigned(blocks), 64 * waves, lds, st>>>(a);
+  const auto go = [&](auto kernel) { kernel<<<unsigned(blocks), 64 * waves, lds, st>>>(a); };
+  if (!whole)
+    go(once ? mx_stream_kernel<DUAL, HALF, true, false>
+            : mx_stream_kernel<DUAL, HALF, false, false>);
   else
-    mx_stream_kernel<DUAL, HALF, false><<<unsigned(blocks), 64 * waves, lds, st>>>(a);
+    go(once ? mx_stream_kernel<DUAL, HALF, true, true>
+            : mx_stream_kernel<DUAL, HALF, false, true>);
   PMOE_LAUNCH_CHECK("mx_stream_kernel");
   return PMOE_OK;
 }
@@ -1307,7 +1188,7 @@ int launch_tile(const MxArgs& a, int max_tiles, hipStream_t st) {
   const int64_t blocks = (int64_t(max_tiles) * ((a.features + kCols - 1) / kCols) + 7) / 8 * 8;
   ProfScope prof_scope(DUAL ? K_MX_GATEUP : K_MX_DOWN, st);
   const int64_t scales = DUAL ? a.s0 | a.s1 : a.s0;
-  if (a.cols % kStep == 0 && (scales | a.expert_bytes) % 16 == 0)
+  if (a.cols % kStretch == 0 && (scales | a.expert_bytes) % 16 == 0)
     mx_tile_kernel<DUAL, true, HALF><<<unsigned(blocks), 64 * kTileWaves, 0, st>>>(a);
   else
     mx_tile_kernel<DUAL, false, HALF><<<unsigned(blocks), 64 * kTileWaves, 0, st>>>(a);
@@ -1364,11 +1245,11 @@ int mx_experts(const MxPlan& p, hipStream_t st) {
   const bool shared = p.kk > p.k;
   const int n_ids = p.n_experts + (shared ? 1 : 0), rows = p.n * p.kk;
   const bool large = p.tile_rows == kTileRows;
-  const bool stream = mx_aligned(g);
+  const bool whole = mx_aligned(g);
   PMOE_REQUIRE(n_ids <= kMaxExperts, "dispatch: experts must be 1..1024");
   {  // a launch holds less than 2^32 threads: the split's, the combine's, the products'
-    const int up_cols = large ? kTileCols / 2 : kSmallCols;
-    const int down_cols = large ? kTileCols : stream ? kStreamRows : kSmallCols;
+    const int up_cols = (large ? kTileCols : kStreamRows) / 2;
+    const int down_cols = large ? kTileCols : kStreamRows;
     const int64_t blocks = std::max((g->inter + up_cols - 1) / up_cols,
                                     (g->hidden + down_cols - 1) / down_cols);
     const int64_t row_blocks = (g->hidden + 2047) / 2048;
@@ -1417,9 +1298,8 @@ int mx_experts(const MxPlan& p, hipStream_t st) {
   a.cols = g->hidden;
   a.pair = p.xpair, a.third = p.xthird, a.ascale = p.xscale, a.asteps = p.xsteps;
   a.hpair = p.hpair, a.hscale = p.hscale;
-  if (int rc = large    ? launch_tile<true, false>(a, p.max_tiles, st)
-               : stream ? launch_stream<true, false>(a, p.max_tiles, once, st)
-                        : launch_small<true, false>(a, p.max_tiles, st))
+  if (int rc = large ? launch_tile<true, false>(a, p.max_tiles, st)
+                     : launch_stream<true, false>(a, p.max_tiles, once, whole, st))
     return rc;
   a.w0 = g->off[PMOE_DOWN_W], a.s0 = g->off[PMOE_DOWN_S];
   a.features = g->hidden;
@@ -1429,12 +1309,10 @@ int mx_experts(const MxPlan& p, hipStream_t st) {
   a.yscale = p.yscale;
   a.past_caches = past_caches(int64_t(rows) * g->hidden);
   if (p.yscale)
-    return large    ? launch_tile<false, true>(a, p.max_tiles, st)
-           : stream ? launch_stream<false, true>(a, p.max_tiles, once, st)
-                    : launch_small<false, true>(a, p.max_tiles, st);
-  return large    ? launch_tile<false, false>(a, p.max_tiles, st)
-         : stream ? launch_stream<false, false>(a, p.max_tiles, once, st)
-                  : launch_small<false, false>(a, p.max_tiles, st);
+    return large ? launch_tile<false, true>(a, p.max_tiles, st)
+                 : launch_stream<false, true>(a, p.max_tiles, once, whole, st);
+  return large ? launch_tile<false, false>(a, p.max_tiles, st)
+               : launch_stream<false, false>(a, p.max_tiles, once, whole, st);
 }
 
 // One token: two launches, no dispatch; out bf16 [hidden] combined (wts given), or
@@ -1476,7 +1354,7 @@ int mx_one(const pmoe_geom* g, const uint8_t* slab, const int32_t* table, int n_
                            st>>>(a, wave_lds);
     PMOE_LAUNCH_CHECK("mx_one_gateup_kernel");
   }
-  const int stretches = (a.inter + kStep - 1) / kStep;
+  const int stretches = (a.inter + kStretch - 1) / kStretch;
   const int items = wts ? a.kk * stretches : stretches;
   const int waves = waves_for(items);
   const int batch = std::min((items + waves - 1) / waves, kOneBatch);
