@@ -188,6 +188,11 @@ __device__ __forceinline__ void split_token(const MxSplit& a, int token, int g, 
     mx_store_pair(a.pair + row * kMxStepPair, g, p0, p1);
     mx_store_third(a.third + row * kMxStepThird, g, p2);
     a.scales[size_t(token) * a.scale_row + mx_scale_at(g)] = uint8_t(s);
+  } else if (token < a.n && g < a.steps * kMxStepGroups) {  // zeros to the end of the step
+    const size_t row = size_t(token) * a.steps;
+    mx_store_pair(a.pair + row * kMxStepPair, g, u32x6{}, u32x6{});
+    mx_store_third(a.third + row * kMxStepThird, g, make_uint4(0, 0, 0, 0));
+    a.scales[size_t(token) * a.scale_row + mx_scale_at(g)] = 127;
   }
   const uint64_t m = __ballot(peak);
   if (token < a.n && (g & 63) == 0) {
@@ -845,12 +850,16 @@ struct Steps {
 // cache four times the accesses and bound the kernel), in an order that keeps the
 // reads back free of bank conflicts (swizzle4).  The next step's loads are in
 // flight while this one's products run.
-// Scales come 16 bytes a row, those of four steps.  BLOCKS: the reduction is
-// whole stretches of 512, so that the weights' lie on 16 bytes too; otherwise
-// theirs are fetched 4 bytes a row for each step (those fetches alone took a
-// sixth of the kernel's time where every step did so).
-template <bool DUAL, bool BLOCKS, bool HALF>
+// Scales come 16 bytes a row, those of four steps.  The weights' do so where the
+// reduction is whole stretches of 512 (kBlocks), so that they lie on 16 bytes;
+// where it is whole steps of 128 they are fetched 4 bytes a row for each step
+// (kWords; those fetches alone took a sixth of the kernel's time where every step
+// did so); otherwise a step's words go through registers, a step ahead, and the
+// last step's groups past the row's end count as zeros (kRegs).
+enum TileScales { kBlocks, kWords, kRegs };
+template <bool DUAL, TileScales SC, bool HALF>
 __global__ __launch_bounds__(64 * kTileWaves, 2) void mx_tile_kernel(const MxArgs a) {
+  constexpr bool BLOCKS = SC == kBlocks;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kTileLds];
   __shared__ unsigned long long s_third;
   __shared__ int32_t s_order[DUAL ? 1 : kTileRows];  // flat rows, for the stores
@@ -890,7 +899,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void mx_tile_kernel(const MxArg
   // wave's own bases; a tile's intermediate rows follow each other, tokens lie
   // anywhere in less than 4 GiB (mx_tile_rows).
   const int lr = lane >> 2, lq = (lane & 3) ^ swizzle4(lr);
-  const int steps = groups / kMxStepGroups;
+  const int steps = (groups + kMxStepGroups - 1) / kMxStepGroups;
   const auto act_row = [&](int row) {
     const int k = row < m ? row : 0;
     return uint32_t(DUAL ? a.order[p0 + k] / a.kk : k);
@@ -936,6 +945,8 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void mx_tile_kernel(const MxArg
       uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)lds)));
   // scales: LDS buffer of the block that a step is in
   const auto scale_lds = [&](int block) { return 2 * kStageBytes + (block & 1) * kScaleBytes; };
+  uint32_t sword = 0;  // kRegs: scales of row 64 wave + lane in the step that is loading
+  const uint8_t* wscale_row = wscale + wscale_off;
   // A step's loads in four parts, so that they can be spread over the products of
   // the step before.
   const auto issue = [&](const Steps& st, int buf, int block, int part) {
@@ -950,8 +961,9 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void mx_tile_kernel(const MxArg
     } else if (part < 3) {
 #pragma unroll
       for (int i = 2 * part - 2; i < 2 * part; ++i)
-        dma16(to + kActBytes + (wave * 4 + i) * 1024, w_off,
-              wbase + size_t(tile_row(4 * wave + i)) * (a.cols / 2) + s * 64);
+        if (SC != kRegs || 4 * s + lq < groups)
+          dma16(to + kActBytes + (wave * 4 + i) * 1024, w_off,
+                wbase + size_t(tile_row(4 * wave + i)) * (a.cols / 2) + s * 64);
     } else {
       if (DUAL && (thirds >> s & 1))
         dma16(to + kActBytes + kWeightBytes + wave * 1024, third_off, a.third + s * kMxStepThird);
@@ -962,7 +974,18 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void mx_tile_kernel(const MxArg
         if constexpr (BLOCKS)
           dma16(sc + kActScaleBytes + wave * 64 * kMxScaleBlock, wscale_off, wscale + at16);
       }
-      if constexpr (!BLOCKS)  // step i of a block: rows' words side by side
+      if constexpr (SC == kRegs) {
+        if (4 * s + 4 <= groups) {
+          __builtin_memcpy(&sword, wscale_row + 4 * s, 4);
+        } else {
+          sword = 0x7f7f7f7f;
+#pragma unroll
+          for (int b = 0; b < 3; ++b)
+            if (4 * s + b < groups)
+              sword = (sword & ~(0xffu << 8 * b)) | uint32_t(wscale_row[4 * s + b]) << 8 * b;
+        }
+      }
+      if constexpr (SC == kWords)  // step i of a block: rows' words side by side
         dma4(sc + kActScaleBytes + (s % kMxScaleSteps) * (kTileCols * 4) + wave * 256, wscale_off,
              wscale + s * 4);
     }
@@ -996,6 +1019,10 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void mx_tile_kernel(const MxArg
   uint32_t sw4[8], sa4[4];  // the lane's scales of a block's steps, this one's lowest
   for (int buf = 0; !todo.done(); buf ^= 1) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if constexpr (SC == kRegs)  // (where kWords' fetches put them)
+      *reinterpret_cast<uint32_t*>(lds + scale_lds(block) + kActScaleBytes +
+                                   (todo.s % kMxScaleSteps) * (kTileCols * 4) + wave * 256 +
+                                   lane * 4) = sword;
     __syncthreads();  // this step is in LDS, and the other buffer has been read
     const bool more = !ahead.done();
     if (more) block_ahead += ahead.fresh() ? 1 : 0;
@@ -1121,8 +1148,13 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void mx_tile_kernel(const MxArg
         mx_split<false>(v, s, h0, h1, none);
         const size_t to = size_t(p0 + row) * mx_steps(a.features);
         mx_store_pair(a.hpair + to * kMxStepPair, f / kMxGroup, h0, h1);
-        a.hscale[size_t(p0 + row) * mx_scale_row(a.features) + mx_scale_at(f / kMxGroup)] =
-            uint8_t(s);
+        uint8_t* hs_row = a.hscale + size_t(p0 + row) * mx_scale_row(a.features);
+        hs_row[mx_scale_at(f / kMxGroup)] = uint8_t(s);
+        if (SC == kRegs && f + kMxGroup == a.features)  // zeros to the end of the step
+          for (int g = a.features / kMxGroup; g % kMxStepGroups; ++g) {
+            mx_store_pair(a.hpair + to * kMxStepPair, g, u32x6{}, u32x6{});
+            hs_row[mx_scale_at(g)] = 127;
+          }
       }
       __syncthreads();
     }
@@ -1183,15 +1215,20 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void mx_tile_kernel(const MxArg
 }
 
 template <bool DUAL, bool HALF>
-int launch_tile(const MxArgs& a, int max_tiles, hipStream_t st) {
+int launch_tile(const MxArgs& a, int max_tiles, bool whole, hipStream_t st) {
   constexpr int kCols = DUAL ? kTileCols / 2 : kTileCols;
   const int64_t blocks = (int64_t(max_tiles) * ((a.features + kCols - 1) / kCols) + 7) / 8 * 8;
   ProfScope prof_scope(DUAL ? K_MX_GATEUP : K_MX_DOWN, st);
   const int64_t scales = DUAL ? a.s0 | a.s1 : a.s0;
-  if (a.cols % kStretch == 0 && (scales | a.expert_bytes) % 16 == 0)
-    mx_tile_kernel<DUAL, true, HALF><<<unsigned(blocks), 64 * kTileWaves, 0, st>>>(a);
+  const auto go = [&](auto kernel) {
+    kernel<<<unsigned(blocks), 64 * kTileWaves, 0, st>>>(a);
+  };
+  if (!whole)
+    go(mx_tile_kernel<DUAL, kRegs, HALF>);
+  else if (a.cols % kStretch == 0 && (scales | a.expert_bytes) % 16 == 0)
+    go(mx_tile_kernel<DUAL, kBlocks, HALF>);
   else
-    mx_tile_kernel<DUAL, false, HALF><<<unsigned(blocks), 64 * kTileWaves, 0, st>>>(a);
+    go(mx_tile_kernel<DUAL, kWords, HALF>);
   PMOE_LAUNCH_CHECK("mx_tile_kernel");
   return PMOE_OK;
 }
@@ -1201,8 +1238,8 @@ int launch_tile(const MxArgs& a, int max_tiles, hipStream_t st) {
 namespace {
 
 // Reductions of whole steps of 128, scales that a lane can fetch four at a time,
-// components within 32-bit offsets of their slot: what the streamed and the large
-// tiles need.
+// components within 32-bit offsets of their slot: where scales need no way through
+// registers, and what the forms for one token take.
 bool mx_aligned(const pmoe_geom* g) {
   if (g->hidden % 128 || g->inter % 128) return false;
   const int comps[] = {PMOE_GATE_S, PMOE_UP_S, PMOE_DOWN_S};
@@ -1227,7 +1264,6 @@ bool mx_aligned(const pmoe_geom* g) {
 //   4096x1536, 8 experts    50: 74 / 97, 100: 121 / 103
 // PMOE_MX_TILE=0 / 1 pins 16 / 128 where the shape allows it (read per call).
 int mx_tile_rows(const pmoe_geom* g, int n, int kk, int n_experts) {
-  if (!mx_aligned(g)) return kFewRows;
   // the tokens' pieces within the large tiles' 32-bit offsets
   if (int64_t(n) * mx_steps(g->hidden) * kMxStepPair >= int64_t(1) << 32) return kFewRows;
   const char* v = getenv("PMOE_MX_TILE");
@@ -1298,7 +1334,7 @@ int mx_experts(const MxPlan& p, hipStream_t st) {
   a.cols = g->hidden;
   a.pair = p.xpair, a.third = p.xthird, a.ascale = p.xscale, a.asteps = p.xsteps;
   a.hpair = p.hpair, a.hscale = p.hscale;
-  if (int rc = large ? launch_tile<true, false>(a, p.max_tiles, st)
+  if (int rc = large ? launch_tile<true, false>(a, p.max_tiles, whole, st)
                      : launch_stream<true, false>(a, p.max_tiles, once, whole, st))
     return rc;
   a.w0 = g->off[PMOE_DOWN_W], a.s0 = g->off[PMOE_DOWN_S];
@@ -1309,9 +1345,9 @@ int mx_experts(const MxPlan& p, hipStream_t st) {
   a.yscale = p.yscale;
   a.past_caches = past_caches(int64_t(rows) * g->hidden);
   if (p.yscale)
-    return large ? launch_tile<false, true>(a, p.max_tiles, st)
+    return large ? launch_tile<false, true>(a, p.max_tiles, whole, st)
                  : launch_stream<false, true>(a, p.max_tiles, once, whole, st);
-  return large ? launch_tile<false, false>(a, p.max_tiles, st)
+  return large ? launch_tile<false, false>(a, p.max_tiles, whole, st)
                : launch_stream<false, false>(a, p.max_tiles, once, whole, st);
 }
 

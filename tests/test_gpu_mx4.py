@@ -259,6 +259,40 @@ def test_tile_forms(monkeypatch, pin, hidden, inter, experts, n, k):
                                        torch.from_numpy(inds).to(DEV)))
 
 
+@pytest.mark.parametrize("pin", ["0", "1", None])
+@pytest.mark.parametrize("hidden,inter,experts,n,k", [
+    (32, 32, 3, 40, 2), (96, 224, 2, 300, 1), (160, 544, 3, 150, 2), (544, 160, 2, 130, 2),
+    (1440, 288, 3, 70, 2), (288, 1440, 2, 17, 2), (8160, 32, 2, 18, 1), (32, 8160, 2, 18, 1),
+    (128, 96, 2, 140, 2), (96, 128, 2, 140, 2)])
+def test_tile_forms_of_ragged_reductions(monkeypatch, pin, hidden, inter, experts, n, k):
+    """Reductions that end inside a step of 128, from one group to the most, both
+    tile heights and what the rule takes: seam and combined outputs, twice the
+    same bits, though what the rows' ends lie on differs between the calls."""
+    if pin is None:
+        monkeypatch.delenv("PMOE_MX_TILE", raising=False)
+    else:
+        monkeypatch.setenv("PMOE_MX_TILE", pin)
+    rng = np.random.default_rng(hidden * 3 + n)
+    L = Layer(hidden, inter, experts, perm=True)
+    x = tokens(rng, n, hidden)
+    inds = rng.integers(0, experts, (n, k)).astype(np.int32)
+    w = rng.random((n, k)).astype(np.float32)
+    t, wt = torch.from_numpy(inds).to(DEV), torch.from_numpy(w).to(DEV)
+    xd = x.double().cpu().numpy()
+    y = K.switch_glu(L.g, L.slab.buf, L.table, experts, x, t)
+    ref, b = L.seam(xd, inds)
+    check(y, ref, b)
+    out = K.moe_experts(L.g, L.slab.buf, L.table, experts, x, t, wt)
+    ref, b = combined(L, xd, inds, w.astype(np.float64))
+    check(out, ref, b)
+    # scratch full of bytes that would be NaN as scales
+    ws = K.moe_workspace(L.g, n, k, 0, experts, x.device)
+    ws.fill_(255)
+    _lib.check(_lib.lib().pmoe_moe_workspace_init(ws.data_ptr(), ws.numel(), K._stream()))
+    assert torch.equal(y, K.switch_glu(L.g, L.slab.buf, L.table, experts, x, t))
+    assert torch.equal(out, K.moe_experts(L.g, L.slab.buf, L.table, experts, x, t, wt))
+
+
 def combined(L, x, inds, w, gate=None):
     y, b = L.seam(x, inds)
     out = (y * w[..., None]).sum(1)
