@@ -560,7 +560,7 @@ int experts_and_combine(const pmoe_geom* g, const uint8_t* slab, const int32_t* 
   const int kk = k + shared;
   if (is_mx(g)) {
     const uint16_t* gate = shared ? shared_gate : nullptr;
-    if (n > 1 || !mx_one_covers(g, kk)) {
+    if (n > 1 || !mx_one_covers(kk)) {
       if (int rc = run_mx(g, slab, table, n_experts, shared_slot, gate, x, inds, n, k, kk, w,
                           nullptr, st))
         return rc;
@@ -677,7 +677,7 @@ extern "C" int pmoe_switch_glu(const pmoe_geom* g, const void* slab, const int32
   MoeWs w;
   pmoe::carve(g, n, k, 0, n_experts, ws, &w);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (n == 1 && pmoe::is_mx(g) && pmoe::mx_one_covers(g, k))
+  if (n == 1 && pmoe::is_mx(g) && pmoe::mx_one_covers(k))
     return pmoe::mx_one(g, static_cast<const uint8_t*>(slab), table, n_experts,
                         static_cast<const uint16_t*>(x), inds, nullptr, k, -1, nullptr, nullptr,
                         w.order, w.h32, static_cast<uint16_t*>(y), st);

@@ -64,7 +64,7 @@ int mx_min_tile_rows();
 int mx_experts(const MxPlan& p, hipStream_t st);
 // One token in two launches, without a dispatch: out bf16 [hidden] combined (wts
 // given) or [k, hidden].  slots [k + 1], h fp32 [k + 1, inter]: scratch.
-bool mx_one_covers(const pmoe_geom* g, int kk);
+bool mx_one_covers(int kk);
 int mx_one(const pmoe_geom* g, const uint8_t* slab, const int32_t* table, int n_experts,
            const uint16_t* x, const int32_t* ids, const float* wts, int k, int shared_slot,
            const uint16_t* shared_gate, float* shared_logit, int32_t* slots, float* h,

@@ -40,6 +40,19 @@ __device__ __forceinline__ const uint8_t* uniform_ptr(const uint8_t* p) {
   return reinterpret_cast<const uint8_t*>(uint64_t(lo) | uint64_t(hi) << 32);
 }
 
+// Four groups' scale bytes, of which `left` are there; 127 (one) for the others.
+__device__ __forceinline__ uint32_t scale_word(const uint8_t* at, int left) {
+  uint32_t v = 0x7f7f7f7f;
+  if (left >= 4) {
+    __builtin_memcpy(&v, at, 4);
+  } else {
+#pragma unroll
+    for (int b = 0; b < 3; ++b)
+      if (b < left) v = (v & ~(0xffu << 8 * b)) | uint32_t(at[b]) << 8 * b;
+  }
+  return v;
+}
+
 // acc += W (16 rows x 128) times a piece of 16 activation rows; sw, sp: the
 // lane's scale bytes.
 __device__ __forceinline__ void mx_mma(f32x4& acc, const uint4& w, int sw, const uint32_t (&p)[6],
@@ -387,21 +400,11 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void mx_stream_kernel(const MxAr
       }
       sa4 = *reinterpret_cast<const uint32_t*>(ascale + (j >> 1) * kMxScaleBlock);
     }
-    uint32_t sword[2] = {0x7f7f7f7f, 0x7f7f7f7f};
-    if constexpr (!WHOLE) {
+    uint32_t sword[2];
+    if constexpr (!WHOLE)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int g = 8 * j + 4 * i;
-        if (g + 4 <= groups) {
-          __builtin_memcpy(&sword[i], sbase + g, 4);
-        } else {
-#pragma unroll
-          for (int b = 0; b < 3; ++b)
-            if (g + b < groups)
-              sword[i] = (sword[i] & ~(0xffu << 8 * b)) | uint32_t(sbase[g + b]) << 8 * b;
-        }
-      }
-    }
+      for (int i = 0; i < 2; ++i)
+        sword[i] = scale_word(sbase + 8 * j + 4 * i, groups - 8 * j - 4 * i);
     // the LDS reads of the step before are done
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
@@ -548,9 +551,11 @@ __device__ __forceinline__ int one_slot(const MxOne& a, int c) {
 // 16 rows x 512 values of a projection into LDS at `to`: 16 lanes side by side on
 // a row's 256 bytes, 4 rows an instruction; then the rows' scales, 4 words each,
 // at to + 4096 (word i of row r at 64 i + 4 r).  In stretch j of `groups` groups,
-// fetched by one wave.
-__device__ __forceinline__ void one_fetch(uint32_t to, const uint8_t* w, const uint8_t* s,
-                                          uint32_t row_bytes, int groups, int j, int lane) {
+// fetched by one wave.  WHOLE as in mx_stream_kernel: otherwise returns the lane's
+// word of scales, which belongs at to + 4096 + 4 lane.
+template <bool WHOLE>
+__device__ __forceinline__ uint32_t one_fetch(uint32_t to, const uint8_t* w, const uint8_t* s,
+                                              uint32_t row_bytes, int groups, int j, int lane) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int row = 4 * i + (lane >> 4);
@@ -560,7 +565,10 @@ __device__ __forceinline__ void one_fetch(uint32_t to, const uint8_t* w, const u
             w + size_t(4 * i) * row_bytes + j * 256);
   }
   const int r = lane & 15, i = lane >> 4;
+  if constexpr (!WHOLE)
+    return scale_word(s + size_t(r) * groups + 16 * j + 4 * i, groups - 16 * j - 4 * i);
   if (16 * j + 4 * i < groups) dma4(to + 4096, uint32_t(r) * groups + 4 * i, s + 16 * j);
+  return 0;
 }
 constexpr int kOneFetch = 4096 + 256;
 // A stretch's pieces in LDS: 16 groups of 64 bytes (p0 and p1 48), their scales
@@ -601,6 +609,7 @@ __device__ __forceinline__ void one_mma(f32x4& acc, const uint8_t* w, const uint
 // in mx_stream_kernel.  Each wave splits its own stretches of x into pieces, a
 // lane a group, while the slot is looked up and its first weights are on their
 // way.  All 16 columns of the products hold the same row.
+template <bool WHOLE>
 __global__ __launch_bounds__(64 * kMaxWaves, 4) void mx_one_gateup_kernel(const MxOne a,
                                                                           int wave_lds) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t dyn[];
@@ -610,7 +619,8 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void mx_one_gateup_kernel(const 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int r = lane & 15, q = lane >> 4;
-  const int groups = a.hidden / kMxGroup, steps = groups / kMxStepGroups;
+  const int groups = a.hidden / kMxGroup;
+  const int steps = (groups + kMxStepGroups - 1) / kMxStepGroups;
   uint8_t* own = dyn + wave * wave_lds;
   uint8_t* pieces = own + kStreamWave;  // [round][8 groups][64 bytes], then their scales
   const int rounds = (steps + 2 * waves - 1) / (2 * waves);
@@ -638,6 +648,9 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void mx_one_gateup_kernel(const 
     const int lp[2] = {(lane & 7) ^ swizzle8(lrow), (lane & 7) ^ swizzle8(lrow + 8)};
     const uint32_t s_off =
         uint32_t(q > 1 ? a.s1 : a.s0) + uint32_t(fb * kCols + 16 * (q & 1) + r) * groups;
+    const uint8_t* srow = base + (q > 1 ? a.s1 : a.s0) +
+                          size_t(fb * kCols + 16 * (q & 1) + r) * groups;
+    uint32_t sword[2];
     const uint32_t own_lds = __builtin_amdgcn_readfirstlane(
         uint32_t(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)own)));
     const auto fetch = [&](int j) {
@@ -646,12 +659,15 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void mx_one_gateup_kernel(const 
       for (int f = 0; f < NF; ++f)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          if (two || lp[i] < 4)
+          if (WHOLE ? two || lp[i] < 4 : 8 * j + lp[i] < groups)
             dma16(own_lds + f * 2048 + i * 1024, lrow * row_bytes + lp[i] * 16,
                   wbase[f] + size_t(8 * i) * row_bytes + j * 128);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        if (i == 0 || two) dma4(own_lds + NF * 2048 + i * 256, s_off + (2 * j + i) * 4, base);
+        if constexpr (!WHOLE)
+          sword[i] = scale_word(srow + 8 * j + 4 * i, groups - 8 * j - 4 * i);
+        else if (i == 0 || two)
+          dma4(own_lds + NF * 2048 + i * 256, s_off + (2 * j + i) * 4, base);
     };
     if (2 * wave < steps) fetch(wave);
     if (has) {
@@ -669,6 +685,9 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void mx_one_gateup_kernel(const 
       mx_split<true>(v, s, p0, p1, p2);
       one_put(pieces, lane, p0, p1, p2);
       pscale[lane] = uint8_t(s);
+    } else if (!WHOLE && (lane >> 3) < rounds) {  // past the row's end
+      one_put(pieces, lane, u32x6{}, u32x6{}, make_uint4(0, 0, 0, 0));
+      pscale[lane] = 127;
     }
     f32x4 acc[NF];
 #pragma unroll
@@ -676,6 +695,10 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void mx_one_gateup_kernel(const 
     int round = 0;
     for (int j = wave; 2 * j < steps; j += waves, ++round) {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      if constexpr (!WHOLE)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          *reinterpret_cast<uint32_t*>(own + NF * 2048 + i * 256 + lane * 4) = sword[i];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         if (2 * j + i >= steps) break;
@@ -734,7 +757,7 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void mx_one_gateup_kernel(const 
 // 16 features of the down projection.  MIX: of the weighted sum over all columns,
 // in fp32 (each wave adds up its own (column, stretch) items, the waves meet in
 // LDS, always in the same order); otherwise of column blockIdx.y.
-template <bool MIX>
+template <bool MIX, bool WHOLE>
 __global__ __launch_bounds__(64 * kMaxWaves, 2) void mx_one_down_kernel(const MxOne a, int batch) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t dyn[];
   const int f0 = blockIdx.x * kOneCols;
@@ -760,15 +783,17 @@ __global__ __launch_bounds__(64 * kMaxWaves, 2) void mx_one_down_kernel(const Mx
   f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
   for (int t0 = wave; t0 < items; t0 += waves * batch) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    for (int b = 0; b < batch; ++b) {
+    uint32_t sword[kOneBatch] = {};
+#pragma unroll
+    for (int b = 0; b < kOneBatch; ++b) {
       const int t = t0 + b * waves;
-      if (t >= items) break;
+      if (b >= batch || t >= items) break;
       const int c = first + t / stretches, j = t % stretches;
       const int slot = __builtin_amdgcn_readlane(my_slot, c);
       if (slot < 0) continue;
       const uint8_t* base = a.slab + size_t(slot) * size_t(a.expert_bytes);
-      one_fetch(own_lds + b * kOneItem, base + a.wd + size_t(f0) * row_bytes,
-                base + a.sd + size_t(f0) * groups, row_bytes, groups, j, lane);
+      sword[b] = one_fetch<WHOLE>(own_lds + b * kOneItem, base + a.wd + size_t(f0) * row_bytes,
+                                  base + a.sd + size_t(f0) * groups, row_bytes, groups, j, lane);
     }
     {  // 16 lanes an item: a group of its column's h each
       const int b = lane >> 4, t = min(t0 + b * waves, items - 1);
@@ -790,10 +815,18 @@ __global__ __launch_bounds__(64 * kMaxWaves, 2) void mx_one_down_kernel(const Mx
           uint8_t* to = own + b * kOneItem + kOneFetch;
           one_put(to, lane & 15, p0, p1, none);
           to[16 * 64 + (lane & 15)] = uint8_t(s);
+        } else if (!WHOLE && held >= 0) {  // past the row's end
+          uint8_t* to = own + b * kOneItem + kOneFetch;
+          one_put(to, lane & 15, u32x6{}, u32x6{}, make_uint4(0, 0, 0, 0));
+          to[16 * 64 + (lane & 15)] = 127;
         }
       }
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    if constexpr (!WHOLE)
+#pragma unroll
+      for (int b = 0; b < kOneBatch; ++b)
+        if (b < batch) *reinterpret_cast<uint32_t*>(own + b * kOneItem + 4096 + lane * 4) = sword[b];
     for (int b = 0; b < batch; ++b) {
       const int t = t0 + b * waves;
       if (t >= items) break;
@@ -974,17 +1007,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void mx_tile_kernel(const MxArg
         if constexpr (BLOCKS)
           dma16(sc + kActScaleBytes + wave * 64 * kMxScaleBlock, wscale_off, wscale + at16);
       }
-      if constexpr (SC == kRegs) {
-        if (4 * s + 4 <= groups) {
-          __builtin_memcpy(&sword, wscale_row + 4 * s, 4);
-        } else {
-          sword = 0x7f7f7f7f;
-#pragma unroll
-          for (int b = 0; b < 3; ++b)
-            if (4 * s + b < groups)
-              sword = (sword & ~(0xffu << 8 * b)) | uint32_t(wscale_row[4 * s + b]) << 8 * b;
-        }
-      }
+      if constexpr (SC == kRegs) sword = scale_word(wscale_row + 4 * s, groups - 4 * s);
       if constexpr (SC == kWords)  // step i of a block: rows' words side by side
         dma4(sc + kActScaleBytes + (s % kMxScaleSteps) * (kTileCols * 4) + wave * 256, wscale_off,
              wscale + s * 4);
@@ -1239,7 +1262,7 @@ namespace {
 
 // Reductions of whole steps of 128, scales that a lane can fetch four at a time,
 // components within 32-bit offsets of their slot: where scales need no way through
-// registers, and what the forms for one token take.
+// registers.
 bool mx_aligned(const pmoe_geom* g) {
   if (g->hidden % 128 || g->inter % 128) return false;
   const int comps[] = {PMOE_GATE_S, PMOE_UP_S, PMOE_DOWN_S};
@@ -1353,7 +1376,7 @@ int mx_experts(const MxPlan& p, hipStream_t st) {
 
 // One token: two launches, no dispatch; out bf16 [hidden] combined (wts given), or
 // [kk, hidden].  Up to 64 columns: a lane looks one up.
-bool mx_one_covers(const pmoe_geom* g, int kk) { return kk <= 64 && mx_aligned(g); }
+bool mx_one_covers(int kk) { return kk <= 64; }
 
 int mx_one(const pmoe_geom* g, const uint8_t* slab, const int32_t* table, int n_experts,
            const uint16_t* x, const int32_t* ids, const float* wts, int k, int shared_slot,
@@ -1376,6 +1399,7 @@ int mx_one(const pmoe_geom* g, const uint8_t* slab, const int32_t* table, int n_
   a.x = x;
   a.hidden = g->hidden, a.inter = g->inter;
   a.h = h, a.out = out;
+  const bool whole = mx_aligned(g);
   const auto waves_for = [](int items) {
     const int rounds = (items + kMaxWaves - 1) / kMaxWaves;
     return (items + rounds - 1) / rounds;
@@ -1386,8 +1410,11 @@ int mx_one(const pmoe_geom* g, const uint8_t* slab, const int32_t* table, int n_
     const int rounds = (steps + waves - 1) / waves;  // 8192 / 256 / 8 at most: a lane a group
     const int wave_lds = (kStreamWave + rounds * 8 * (64 + 1) + 255) / 256 * 256;
     ProfScope prof_scope(K_MX_GATEUP, st);
-    mx_one_gateup_kernel<<<dim3(a.inter / (kStreamRows / 2), a.kk), 64 * waves, waves * wave_lds,
-                           st>>>(a, wave_lds);
+    const auto go = [&](auto kernel) {
+      kernel<<<dim3(a.inter / (kStreamRows / 2), a.kk), 64 * waves, waves * wave_lds, st>>>(
+          a, wave_lds);
+    };
+    go(whole ? mx_one_gateup_kernel<true> : mx_one_gateup_kernel<false>);
     PMOE_LAUNCH_CHECK("mx_one_gateup_kernel");
   }
   const int stretches = (a.inter + kStretch - 1) / kStretch;
@@ -1396,10 +1423,13 @@ int mx_one(const pmoe_geom* g, const uint8_t* slab, const int32_t* table, int n_
   const int batch = std::min((items + waves - 1) / waves, kOneBatch);
   const size_t lds = size_t(waves) * batch * kOneItem;
   ProfScope prof_scope(K_MX_DOWN, st);
+  const auto go = [&](auto kernel) {
+    kernel<<<dim3(a.hidden / kOneCols, wts ? 1 : a.kk), 64 * waves, lds, st>>>(a, batch);
+  };
   if (wts)
-    mx_one_down_kernel<true><<<a.hidden / kOneCols, 64 * waves, lds, st>>>(a, batch);
+    go(whole ? mx_one_down_kernel<true, true> : mx_one_down_kernel<true, false>);
   else
-    mx_one_down_kernel<false><<<dim3(a.hidden / kOneCols, a.kk), 64 * waves, lds, st>>>(a, batch);
+    go(whole ? mx_one_down_kernel<false, true> : mx_one_down_kernel<false, false>);
   PMOE_LAUNCH_CHECK("mx_one_down_kernel");
   return PMOE_OK;
 }

@@ -293,6 +293,28 @@ def test_tile_forms_of_ragged_reductions(monkeypatch, pin, hidden, inter, expert
     assert torch.equal(out, K.moe_experts(L.g, L.slab.buf, L.table, experts, x, t, wt))
 
 
+@pytest.mark.parametrize("hidden,inter,experts,k", [
+    (32, 32, 3, 2), (96, 224, 4, 3), (160, 544, 9, 8), (544, 160, 2, 1), (1440, 288, 3, 2),
+    (288, 1440, 5, 4), (8160, 32, 2, 1), (32, 8160, 2, 2), (128, 96, 70, 60), (96, 4128, 4, 3)])
+def test_one_token_of_ragged_reductions(hidden, inter, experts, k):
+    """Both launches of one token where the reductions end inside a step of 128."""
+    rng = np.random.default_rng(hidden * 5 + inter)
+    L = Layer(hidden, inter, experts, 1, perm=True)
+    x = tokens(rng, 1, hidden)
+    inds = rng.permutation(experts)[None, :k].astype(np.int32)
+    if k > 2:
+        inds[0, 1] = -1
+    w = rng.random((1, k)).astype(np.float32)
+    gate = bf16(rng.standard_normal((1, hidden)) * 0.05)
+    t, wt = torch.from_numpy(inds).to(DEV), torch.from_numpy(w).to(DEV)
+    xd = x.double().cpu().numpy()
+    ref, b = L.seam(xd, inds)
+    check(K.switch_glu(L.g, L.slab.buf, L.table, experts, x, t), ref, b)
+    out = K.moe_experts(L.g, L.slab.buf, L.table, experts, x, t, wt, L.shared_slot, gate)
+    ref, b = combined(L, xd, inds, w.astype(np.float64), gate.double().cpu().numpy())
+    check(out, ref, b)
+
+
 def combined(L, x, inds, w, gate=None):
     y, b = L.seam(x, inds)
     out = (y * w[..., None]).sum(1)
