@@ -8,6 +8,15 @@
 // (mx_pieces.h), two products for each step, three for the few steps in which
 // a value stands out; the sums are fp32.
 //
+// Three forms, by the rows of the call:
+//   one token     two launches without a dispatch: gate/up from x itself, and the
+//                 down projection with the columns' weighted sum inside
+//   few rows an   dispatch and activation pieces in one launch (mx_prepare_kernel),
+//   expert        tiles of 16 rows bound by the weights' stream, a combine
+//   many          tiles of 128 rows bound by the matrix instructions and the loads
+//                 beside them
+// The line between the last two stands at mx_tile_rows.
+//
 // An activation that is infinite or NaN, or an intermediate that leaves fp32,
 // makes the outputs of its row NaN.
 #include <hip/hip_fp16.h>
@@ -109,7 +118,9 @@ __device__ __forceinline__ uint32_t half_wave_max(uint32_t v) {
 inline bool past_caches(int64_t values) { return values >= int64_t(128) << 20; }
 
 // out[n] = bf16(fma over k of weight * y, then the shared expert's times 1 or
-// sigmoid(shared_logit[n])), in column order; 8 features a thread.
+// sigmoid(shared_logit[n])), in column order; 8 features a thread.  Bound by HBM:
+// 16384 tokens x 8 columns x 4096 features 195 us (6.2 TB/s; 242 with ordinary loads,
+// one column at a time); of few tokens by its launch and two rounds of loads (5 us).
 template <bool PAST>
 __global__ __launch_bounds__(256) void mx_combine_kernel(
     const uint16_t* __restrict__ y, const uint8_t* __restrict__ yscale,
@@ -174,6 +185,8 @@ struct MxSplit {
 // A token by 256 threads, a lane a group: its pieces, scales and the mask of the
 // 128-wide steps that hold a third piece (16 bits a wave), the shared expert's gate
 // logit, the zero rows of ids that are dropped.  s_sum: 4 floats of the token's.
+// 16384 x 4096: 134 MB in, 280 MB out, 48 us.  Splitting in the products instead
+// would repeat these ~20 operations a value for every block of features.
 __device__ __forceinline__ void split_token(const MxSplit& a, int token, int g, float* s_sum) {
   bool peak = false;
   float dot = 0.0f;
@@ -238,7 +251,8 @@ __global__ __launch_bounds__(256) void mx_split_kernel(const MxSplit a) {
 }
 
 // The dispatch of a small call beside its split: block 0 dispatches, the others
-// take four tokens each.
+// take four tokens each.  5 us for 24 rows, 7 for 800: the dispatching block's
+// barriers, under which the split hides (two launches took 4 us more).
 struct MxDispatch {
   IdSrc src;
   int rows, n_ids;
@@ -308,7 +322,9 @@ constexpr int kStreamWave = kStreamRows * 128 + 2 * kStreamRows * 4;  // LDS of 
 // bytes go straight into its own LDS, 8 lanes side by side on a row's 128 bytes,
 // so that nothing waits for registers and the fetches are whole lines; two
 // blocks a CU keep 136 KB in flight.  (Loads into registers in the products' own
-// lane order, 16 bytes of 64 different rows an instruction, reached 3 TB/s.)
+// lane order, 16 bytes of 64 different rows an instruction, reached 3 TB/s.)  7168x2048
+// experts, 3 tokens: 573 MB in 76 + 39 us, 5.0 TB/s; 4096x1536, 100 tokens seam: 435 MB
+// in 64 + 33, 4.5 TB/s; 2048x512, 29 tokens: 375 MB in 55 + 25, 4.7 TB/s.
 // ONCE: an expert has one tile on average, and its weights need no place in the
 // caches (us, gate/up + down, without / with it: 4096x1536 8 tokens 66 + 36 / 62 + 33,
 // 7168x2048 3 tokens 80 + 42 / 76 + 40).
@@ -608,7 +624,9 @@ __device__ __forceinline__ void one_mma(f32x4& acc, const uint8_t* w, const uint
 // h[c, f] = silu(gate) * up for 32 features of one column, the weights streamed as
 // in mx_stream_kernel.  Each wave splits its own stretches of x into pieces, a
 // lane a group, while the slot is looked up and its first weights are on their
-// way.  All 16 columns of the products hold the same row.
+// way.  All 16 columns of the products hold the same row.  4096x1536, 8 columns:
+// 53 MB in 13.0 us, 4.1 TB/s: the two lookups, then two rounds of loads a wave (16
+// features a block were slower).
 template <bool WHOLE>
 __global__ __launch_bounds__(64 * kMaxWaves, 4) void mx_one_gateup_kernel(const MxOne a,
                                                                           int wave_lds) {
@@ -756,7 +774,9 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void mx_one_gateup_kernel(const 
 
 // 16 features of the down projection.  MIX: of the weighted sum over all columns,
 // in fp32 (each wave adds up its own (column, stretch) items, the waves meet in
-// LDS, always in the same order); otherwise of column blockIdx.y.
+// LDS, always in the same order); otherwise of column blockIdx.y.  4096x1536, 8
+// columns: 27 MB in 8.9 us, every load of a block in flight at once; what is left is
+// the launch, the slots' lookup and the sum at the end.
 template <bool MIX, bool WHOLE>
 __global__ __launch_bounds__(64 * kMaxWaves, 2) void mx_one_down_kernel(const MxOne a, int batch) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t dyn[];
@@ -883,6 +903,12 @@ struct Steps {
 // cache four times the accesses and bound the kernel), in an order that keeps the
 // reads back free of bank conflicts (swizzle4).  The next step's loads are in
 // flight while this one's products run.
+// 4096x1536, 16384 tokens x 8 columns: gate/up 2.1 to 2.2 ms, down 1.2 (1.5 and 1.35
+// PFLOP/s of the layer's products, twice that and the third pieces on the matrix
+// units).  Gate/up without its loads takes 1.74 ms, near the 1.63 of its matrix
+// instructions alone, and the loads without the products 1.64: what is left is
+// where one waits for the other.  The down projection's 12 steps leave a third of
+// its time to the first loads and the stores.
 // Scales come 16 bytes a row, those of four steps.  The weights' do so where the
 // reduction is whole stretches of 512 (kBlocks), so that they lie on 16 bytes;
 // where it is whole steps of 128 they are fetched 4 bytes a row for each step
@@ -1285,7 +1311,12 @@ bool mx_aligned(const pmoe_geom* g) {
 //   2048x768, 128 experts   9: 94 / 106, 13: 105 / 107, 19: 134 / 114
 //   1024x512, 32 experts    50: 37 / 46, 75: 47 / 48, 100: 55 / 50
 //   4096x1536, 8 experts    50: 74 / 97, 100: 121 / 103
-// PMOE_MX_TILE=0 / 1 pins 16 / 128 where the shape allows it (read per call).
+// Reductions that are no whole steps of 128 have dearer large tiles (their scales
+// go through registers) and pay from 18:
+//   4128x1568, 128 experts  14: 535 / 644, 20: 604 / 657, 62: 1372 / 720
+//   2880x2880, 32 experts   12: 162 / 194, 19: 197 / 197
+//   1056x480, 32 experts    50: 43 / 44, 100: 68 / 47
+// PMOE_MX_TILE=0 / 1 pins 16 / 128 (read per call).
 int mx_tile_rows(const pmoe_geom* g, int n, int kk, int n_experts) {
   // the tokens' pieces within the large tiles' 32-bit offsets
   if (int64_t(n) * mx_steps(g->hidden) * kMxStepPair >= int64_t(1) << 32) return kFewRows;
@@ -1295,7 +1326,8 @@ int mx_tile_rows(const pmoe_geom* g, int n, int kk, int n_experts) {
   const int64_t blocks =
       (n_experts + rows / kTileRows) * ((g->inter + kTileCols / 2 - 1) / (kTileCols / 2));
   constexpr int64_t kFull = 384;
-  return rows * std::min(blocks, kFull) >= 12 * kFull * n_experts ? kTileRows : kFewRows;
+  const int64_t least = (mx_aligned(g) ? 12 : 18) * kFull * n_experts;
+  return rows * std::min(blocks, kFull) >= least ? kTileRows : kFewRows;
 }
 int mx_min_tile_rows() { return kFewRows; }
 

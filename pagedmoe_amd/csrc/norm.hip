@@ -16,6 +16,10 @@
 // holds 8 consecutive elements (16 or 32 bytes a load) of up to 8
 // stretches; the two sums of a row go through a wave's lanes and then LDS.  Rows
 // that are no multiple of 8 long or not on 16 bytes go element by element.
+// Join of 16384 x 4096 bf16 with a gate per element and both norms: 671 MB in 113
+// us, 5.9 TB/s; of 1000 rows with 10 slots of 2048: 53 MB in 10.9.  Few rows are
+// bound by latency: norm of one row of 4096 2.4 us, join of 5 rows of 7168 7.6
+// (six rounds of dependent loads and two sums).
 #include <type_traits>
 
 #include "pmoe_internal.h"

@@ -4,8 +4,8 @@ Counterpart of the reference's ``SlabStore`` (slab.py:82-183).  The reference
 keeps one ``[slots, *expert_shape]`` array per component in unified memory
 and preads into it.  Here a slab is ONE device allocation of
 ``slots * expert_bytes`` bytes laid out expert-major: slot s holds the nine
-components of one expert back to back (``pmoe_geom.off``; six in the microscaled 4-bit format, group 32,
-which has no biases), so a miss is a
+components of one expert back to back (``pmoe_geom.off``; six in the
+microscaled 4-bit format, group 32, which has no biases), so a miss is a
 single contiguous host->HBM copy and every kernel addresses an expert as
 ``base + slot * expert_bytes``.  ``compute(name)`` still hands out the
 reference's ``[slots, *shape]`` view of one component (a strided view, no
