@@ -18,8 +18,9 @@
 // that are no multiple of 8 long or not on 16 bytes go element by element.
 // Join of 16384 x 4096 bf16 with a gate per element and both norms: 671 MB in 113
 // us, 5.9 TB/s; of 1000 rows with 10 slots of 2048: 53 MB in 10.9.  Few rows are
-// bound by latency: norm of one row of 4096 2.4 us, join of 5 rows of 7168 7.6
-// (six rounds of dependent loads and two sums).
+// bound by latency: norm of one row of 4096 2.4 us, join of 5 rows of 7168 fp32 4.4
+// (rounds of loads between two sums; asking for everything before the first sum made
+// 64 rows no faster and 16384 bf16 rows 111 -> 131, by its registers).
 #include <type_traits>
 
 #include "pmoe_internal.h"
@@ -113,18 +114,54 @@ __device__ __forceinline__ void put1(void* base, bool f32, size_t at, float v) {
     static_cast<uint16_t*>(base)[at] = f2bf(v);
 }
 
-// The block's sum of v, in an order that depends on nothing but its threads.
-template <int T>
-__device__ __forceinline__ float block_sum(float v, float* s) {
-  v = wave_sum_bfly(v);
-  if constexpr (T > 64) {
-    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = 0.0f;
+// a + the same of the lane 32 (16) away, for a and b at once: lanes of the lower
+// half (of even rows of 16) end with a's sums, the others with b's.
+__device__ __forceinline__ float fold32(float a, float b) {
+  const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false,
+                                                  false);
+  return __uint_as_float(t[0]) + __uint_as_float(t[1]);
+}
+__device__ __forceinline__ float fold16(float a, float b) {
+  const auto t = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false,
+                                                  false);
+  return __uint_as_float(t[0]) + __uint_as_float(t[1]);
+}
+__device__ __forceinline__ float sum16(float v) {  // over a row of 16 lanes
+  v += xor_lane<8>(v);
+  v += xor_lane<4>(v);
+  v += xor_lane<2>(v);
+  return v + xor_lane<1>(v);
+}
+
+// The block's sum of v, whose v[j] are of stretch j: the sums of 512 elements that
+// a wave holds of a stretch, one after the other, so that it does not depend on how
+// many threads hold the row.  A wave folds up to four stretches at once.
+template <int T, int NV = 1>
+__device__ __forceinline__ float block_sum(const float (&v)[NV], float* s) {
+  constexpr int W = T / 64;
+  const int lane = threadIdx.x & 63;
+  float* to = s + (threadIdx.x >> 6);
+  if constexpr (NV == 1) {
+    const float u = fold32(v[0], v[0]);
+    const float p = sum16(fold16(u, u));
+    if constexpr (W == 1) return p;
+    if (lane == 0) *to = p;
+  } else if constexpr (NV == 2) {
+    const float u = fold32(v[0], v[1]);
+    const float p = sum16(fold16(u, u));
+    if ((lane & 31) == 0) to[W * (lane >> 5)] = p;
+  } else {
 #pragma unroll
-    for (int i = 0; i < T / 64; ++i) v += s[i];
+    for (int j = 0; j < NV; j += 4) {
+      const float p = sum16(fold16(fold32(v[j], v[j + 1]), fold32(v[j + 2], v[j + 3])));
+      if ((lane & 15) == 0) to[W * (j + (lane >> 5) + (lane >> 3 & 2))] = p;
+    }
   }
-  return v;
+  __syncthreads();
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV * W; ++i) sum += s[i];
+  return sum;
 }
 
 // 1 / sqrt(mean + eps)
@@ -138,10 +175,10 @@ template <int T, int NV, bool NT>
 __global__ __launch_bounds__(T) void norm_kernel(const void* x, int x_f32, const void* weight,
                                                  int w_f32, int d, float eps, float offset,
                                                  uint16_t* h) {
-  __shared__ float s[T / 64];
+  __shared__ float s[NV * T / 64];
   const size_t row = size_t(blockIdx.x) * d;
   float v[NV][8];
-  float sum = 0.0f;
+  float sum[NV] = {};
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int c = (j * T + int(threadIdx.x)) * 8;
@@ -152,7 +189,7 @@ __global__ __launch_bounds__(T) void norm_kernel(const void* x, int x_f32, const
     const int c = (j * T + int(threadIdx.x)) * 8;
     if (c < d)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(v[j][i], v[j][i], sum);
+      for (int i = 0; i < 8; ++i) sum[j] = __builtin_fmaf(v[j][i], v[j][i], sum[j]);
   }
   const float r = inv_rms(block_sum<T>(sum, s), d, eps);
 #pragma unroll
@@ -169,7 +206,7 @@ __global__ __launch_bounds__(T) void norm_kernel(const void* x, int x_f32, const
 
 template <int T, int NV, bool NT>
 __global__ __launch_bounds__(T) void join_kernel(const JoinArgs a) {
-  __shared__ float s[2][T / 64];
+  __shared__ float s[2][NV * T / 64];
   const int d = a.d;
   const size_t n = blockIdx.x;
   const size_t row = n * d;
@@ -200,13 +237,13 @@ __global__ __launch_bounds__(T) void join_kernel(const JoinArgs a) {
     }
   }
   if (a.post) {
-    float sum = 0.0f;
+    float sum[NV] = {};
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * T + int(threadIdx.x)) * 8;
       if (c < d)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(y[j][i], y[j][i], sum);
+        for (int i = 0; i < 8; ++i) sum[j] = __builtin_fmaf(y[j][i], y[j][i], sum[j]);
     }
     const float r = inv_rms(block_sum<T>(sum, s[0]), d, a.eps);
 #pragma unroll
@@ -222,7 +259,7 @@ __global__ __launch_bounds__(T) void join_kernel(const JoinArgs a) {
   const float tg = a.gate_kind == PMOE_GATE_TOKEN
                        ? gate_act(get1(a.gate, a.gate_f32, n), a.gate_sigmoid)
                        : 1.0f;
-  float sum = 0.0f;
+  float sum[NV] = {};
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int c = (j * T + int(threadIdx.x)) * 8;
@@ -241,7 +278,7 @@ __global__ __launch_bounds__(T) void join_kernel(const JoinArgs a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       y[j][i] = __builtin_fmaf(a.residual_scale, res[i], a.branch_scale * y[j][i]);
-      sum = __builtin_fmaf(y[j][i], y[j][i], sum);
+      sum[j] = __builtin_fmaf(y[j][i], y[j][i], sum[j]);
     }
     put8<NT>(a.out, a.stream_f32, row + c, y[j]);
   }
@@ -265,10 +302,10 @@ __global__ __launch_bounds__(256) void norm_any_kernel(const void* x, int x_f32,
                                                        uint16_t* h) {
   __shared__ float s[4];
   const size_t row = size_t(blockIdx.x) * d;
-  float sum = 0.0f;
+  float sum[1] = {};
   for (int c = threadIdx.x; c < d; c += 256) {
     const float v = get1(x, x_f32, row + c);
-    sum = __builtin_fmaf(v, v, sum);
+    sum[0] = __builtin_fmaf(v, v, sum[0]);
   }
   const float r = inv_rms(block_sum<256>(sum, s), d, eps);
   for (int c = threadIdx.x; c < d; c += 256)
@@ -301,14 +338,14 @@ __global__ __launch_bounds__(256) void join_any_kernel(const JoinArgs a) {
   const size_t row = n * d;
   float rp = 1.0f;
   if (a.post) {
-    float sum = 0.0f;
+    float sum[1] = {};
     for (int c = threadIdx.x; c < d; c += 256) {
       const float y = branch(a, n, c);
-      sum = __builtin_fmaf(y, y, sum);
+      sum[0] = __builtin_fmaf(y, y, sum[0]);
     }
     rp = inv_rms(block_sum<256>(sum, s[0]), d, a.eps);
   }
-  float sum = 0.0f;
+  float sum[1] = {};
 #pragma unroll
   for (int j = 0; j < kEach; ++j) {
     const int c = j * 256 + int(threadIdx.x);
@@ -323,7 +360,7 @@ __global__ __launch_bounds__(256) void join_any_kernel(const JoinArgs a) {
                     a.gate_sigmoid);
     y = __builtin_fmaf(a.residual_scale, get1(a.residual, a.stream_f32, row + c),
                        a.branch_scale * y);
-    sum = __builtin_fmaf(y, y, sum);
+    sum[0] = __builtin_fmaf(y, y, sum[0]);
     put1(a.out, a.stream_f32, row + c, y);
     keep[j] = y;
   }
@@ -344,20 +381,36 @@ bool on16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 // next kernel finds them there.
 constexpr int64_t kPastCaches = int64_t(64) << 20;
 
-// go(threads, stretches): a wave for rows of up to 512 elements, then 256
-// threads of as many stretches as the row needs.
+// Rows up to which a row gets more threads than it needs.  us, more / fewest, bf16
+// with a gate per element and both norms:
+//   4096    64 rows 4.0 / 5.2   512: 5.9 / 6.7   1024: 10.0 / 9.7   16384: 129 / 111
+//   7168    64: 4.9 / 8.2   512: 9.4 / 11.6   1024: 16.6 / 16.5   2048: 29.5 / 28.9
+//   12288   64: 6.1 / 12.2   512: 13.4 / 19   1024: 23 / 25   2048: 43 / 46
+constexpr int kFewRows = 512;
+
+// go(threads, stretches) for n rows of d: few rows get as many threads as pay, for
+// the shortest way through them, many the fewest that hold a row (the same sums).
 template <class Go>
-void by_width(int d, Go go) {
+void by_width(int n, int d, Go go) {
+  const bool few = n <= kFewRows;
+  const auto with = [&](auto narrow_stretches, auto threads, auto stretches) {
+    if (few)
+      go(threads, stretches);
+    else
+      go(std::integral_constant<int, 256>{}, narrow_stretches);
+  };
+  constexpr std::integral_constant<int, 1> one{};
+  constexpr std::integral_constant<int, 2> two{};
   if (d <= 512)
-    go(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
+    go(std::integral_constant<int, 64>{}, one);
   else if (d <= 2048)
-    go(std::integral_constant<int, 256>{}, std::integral_constant<int, 1>{});
+    go(std::integral_constant<int, 256>{}, one);
   else if (d <= 4096)
-    go(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
+    with(two, std::integral_constant<int, 512>{}, one);
   else if (d <= 8192)
-    go(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
+    with(std::integral_constant<int, 4>{}, std::integral_constant<int, 1024>{}, one);
   else
-    go(std::integral_constant<int, 256>{}, std::integral_constant<int, 8>{});
+    with(std::integral_constant<int, 8>{}, std::integral_constant<int, 1024>{}, two);
 }
 
 bool stream_dtype(int t) { return t == PMOE_F32 || t == PMOE_BF16; }
@@ -385,7 +438,7 @@ extern "C" int pmoe_block_norm(const void* x, int x_dtype, const void* weight, i
   uint16_t* out = static_cast<uint16_t*>(h);
   const int xf = x_dtype == PMOE_F32, wf = weight_dtype == PMOE_F32;
   if (hidden % 8 == 0 && on16(x) && on16(weight) && on16(h))
-    by_width(hidden, [&](auto t, auto nv) {
+    by_width(n, hidden, [&](auto t, auto nv) {
       constexpr int T = decltype(t)::value, NV = decltype(nv)::value;
       if (int64_t(n) * hidden * 2 >= kPastCaches)
         norm_kernel<T, NV, true><<<n, T, 0, st>>>(x, xf, weight, wf, hidden, eps, off, out);
@@ -446,7 +499,7 @@ extern "C" int pmoe_block_join(const pmoe_join* j, const void* residual, const v
   const bool gate_ok = j->gate_kind == PMOE_GATE_TOKEN || on16(gate);
   if (hidden % 8 == 0 && on16(residual) && on16(y) && on16(shared_y) && on16(post_weight) &&
       on16(next_weight) && on16(out) && on16(h) && gate_ok)
-    by_width(hidden, [&](auto t, auto nv) {
+    by_width(n, hidden, [&](auto t, auto nv) {
       constexpr int T = decltype(t)::value, NV = decltype(nv)::value;
       if (int64_t(n) * hidden * (a.stream_f32 ? 4 : 2) >= kPastCaches)
         join_kernel<T, NV, true><<<n, T, 0, st>>>(a);

@@ -165,6 +165,20 @@ def test_rows_off_16_bytes_give_the_same_rows():
         check(b)
 
 
+@pytest.mark.parametrize("d", [8, 512, 520, 2048, 2056, 4096, 4104, 7168, 8192, 8200, 12288, 16384])
+def test_rows_do_not_depend_on_their_number(d):
+    """One row, few and many take different numbers of threads: the same bits."""
+    a = make(700, d, 2, torch.bfloat16, torch.bfloat16, "element", True, True, 0, 3)
+    out, h = run(a)
+    nh = K.block_norm(a["residual"], a["next_weight"])
+    for r0, r1 in ((0, 1), (5, 517), (699, 700)):
+        part = {k: v[r0:r1].contiguous() if torch.is_tensor(v) and v.dim() >= 2 else v
+                for k, v in a.items()}
+        o, hh = run(part)
+        assert torch.equal(out[r0:r1], o) and torch.equal(h[r0:r1], hh)
+        assert torch.equal(nh[r0:r1], K.block_norm(part["residual"], a["next_weight"]))
+
+
 @pytest.mark.parametrize("stream", [torch.bfloat16, torch.float32])
 def test_past_the_caches(stream):
     """Results of more than 64 MiB, in place too: the rows that shorter calls give."""
