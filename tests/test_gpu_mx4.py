@@ -496,6 +496,61 @@ def test_captured_and_replayed(n):
         assert torch.equal(y, y2) and torch.equal(out, out2), r
 
 
+def test_two_graphs_share_the_workspace():
+    """Graphs of different calls and shapes (one token, few rows, several dispatch
+    launches, a ragged reduction), replayed in turn with eager calls between."""
+    rng = np.random.default_rng(3)
+    calls = []
+    for hidden, inter, n in ((512, 256, 1), (512, 256, 9), (96, 160, 33), (512, 256, 400)):
+        L = Layer(hidden, inter, 6, 1)
+        x = tokens(rng, n, hidden)
+        inds = torch.from_numpy(rng.integers(-1, 6, (n, 4)).astype(np.int32)).to(DEV)
+        w = torch.rand(n, 4, device=DEV)
+        calls.append((L, x, lambda L=L, x=x, i=inds, w=w: (
+            K.switch_glu(L.g, L.slab.buf, L.table, 6, x, i),
+            K.moe_experts(L.g, L.slab.buf, L.table, 6, x, i, w, 6))))
+    for _, _, go in reversed(calls):  # the largest workspace first
+        go()
+    graphs = []
+    for _, _, go in calls:
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = go()
+        graphs.append((graph, outs))
+    for r in range(3):
+        for _, x, _ in calls:
+            x.copy_(tokens(rng, *x.shape))
+        for i in rng.permutation(len(calls)):
+            graphs[i][0].replay()
+            if r == 1:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        for (_, _, go), (_, outs) in zip(calls, graphs):
+            assert all(torch.equal(a, b) for a, b in zip(outs, go())), r
+
+
+def test_two_calls_at_once():
+    """Calls on two streams at once, each with a workspace of its own."""
+    import ctypes
+    rng = np.random.default_rng(4)
+    L = Layer(512, 256, 8)
+    inds = torch.from_numpy(rng.integers(0, 8, (150, 4)).astype(np.int32)).to(DEV)
+    xs = [tokens(rng, 150, 512) for _ in range(2)]
+    want = [K.switch_glu(L.g, L.slab.buf, L.table, 8, x, inds) for x in xs]
+    ws = [K.moe_workspace(L.g, 150, 4, 0, 8, x.device, fresh=True) for x in xs]
+    ys = [torch.empty_like(y) for y in want]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(10):
+        for x, w, y, st in zip(xs, ws, ys, streams):
+            _lib.check(_lib.lib().pmoe_switch_glu(
+                ctypes.byref(L.g), L.slab.buf.data_ptr(), L.table.data_ptr(), 8, x.data_ptr(),
+                inds.data_ptr(), 150, 4, y.data_ptr(), w.data_ptr(), w.numel(), st.cuda_stream))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, ys))
+
+
 def test_modules_resident_and_paged():
     """QuantizedSwitchGLU(group=32) under a block, resident, then with its
     experts paged through a slab that holds a part of them: the same bits for
