@@ -67,7 +67,7 @@ def _same_device(a, b, name):
 def _need(t, dtype, name, ndim=None):
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a tensor")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise ValueError(f"{name}: must be a device tensor (got {t.device})")
     if t.dtype != dtype:
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
@@ -361,28 +361,37 @@ def workspace_error(ws: torch.Tensor) -> int:
     return int(err.value)
 
 
-def _table_ptr(table):
+def _table_ptr(table, n_experts: int = 0):
     if isinstance(table, torch.Tensor):
         _need(table, torch.int32, "table", 1)
-        return _ptr(table)
-    return ctypes.c_void_p(int(table))
+        if table.numel() < n_experts:
+            raise ValueError(f"table holds {table.numel()} of {n_experts} experts")
+        return table.data_ptr()
+    return int(table)
+
+
+def _rows_of(x, n, g, inds):
+    """x is bf16 [n, hidden] beside inds: says what is not."""
+    _need(x, torch.bfloat16, "x", 2)
+    if x.shape != (n, g.hidden):
+        raise ValueError(f"x must be [{n}, {g.hidden}], got {tuple(x.shape)}")
+    _same_device(inds, x, "x")
 
 
 def switch_glu(g: Geom, slab: torch.Tensor, table, n_experts: int, x: torch.Tensor,
                inds: torch.Tensor) -> torch.Tensor:
     """y [N, K, D] bf16: row (n, k) through the expert in slot table[inds[n, k]]."""
-    _need(x, torch.bfloat16, "x", 2)
     _need(inds, torch.int32, "inds", 2)
     n, k = inds.shape
-    if x.shape != (n, g.hidden):
-        raise ValueError(f"x must be [{n}, {g.hidden}], got {tuple(x.shape)}")
+    if not _fits(x, torch.bfloat16, (n, g.hidden), inds.get_device()):
+        _rows_of(x, n, g, inds)
     y = x.new_empty((n, k, g.hidden))
     if n == 0:
         return y
     ws = moe_workspace(g, n, k, 0, n_experts, x.device)
-    check(lib().pmoe_switch_glu(ctypes.byref(g), _ptr(slab), _table_ptr(table), n_experts,
-                                _ptr(x), _ptr(inds), n, k, _ptr(y), _ptr(ws), ws.numel(),
-                                _stream()), "pmoe_switch_glu")
+    check(lib().pmoe_switch_glu(ctypes.byref(g), _ptr(slab), _table_ptr(table, n_experts),
+                                n_experts, x.data_ptr(), inds.data_ptr(), n, k, y.data_ptr(),
+                                ws.data_ptr(), ws.numel(), _stream()), "pmoe_switch_glu")
     return y
 
 
@@ -398,18 +407,23 @@ def count_missing(table, ids: torch.Tensor, n_experts: int, counter: torch.Tenso
 def moe_experts(g: Geom, slab, table, n_experts: int, x, inds, weights, shared_slot: int = -1,
                 shared_gate=None) -> torch.Tensor:
     """out [N, D] bf16 = sum_k w[n,k] FFN_{inds[n,k]}(x[n]) (+ shared)."""
-    _need(x, torch.bfloat16, "x", 2)
     _need(inds, torch.int32, "inds", 2)
-    _need(weights, torch.float32, "weights", 2)
     n, k = inds.shape
-    out = torch.empty((n, g.hidden), dtype=torch.bfloat16, device=x.device)
+    dev = inds.get_device()
+    if not _fits(x, torch.bfloat16, (n, g.hidden), dev):
+        _rows_of(x, n, g, inds)
+    if not _fits(weights, torch.float32, (n, k), dev):
+        _like(weights, inds, (n, k), "weights", torch.float32)
+    if shared_gate is not None and shared_gate.numel() != g.hidden:
+        raise ValueError(f"shared_gate must hold {g.hidden} values, got {shared_gate.numel()}")
+    out = torch.empty_like(x)
     if n == 0:
         return out
     ws = moe_workspace(g, n, k, int(shared_slot >= 0), n_experts, x.device)
-    check(lib().pmoe_moe_experts(ctypes.byref(g), _ptr(slab), _table_ptr(table), n_experts,
-                                 _ptr(x), _ptr(inds), _ptr(weights), n, k, int(shared_slot),
-                                 _ptr(shared_gate), _ptr(out), _ptr(ws), ws.numel(), _stream()),
-          "pmoe_moe_experts")
+    check(lib().pmoe_moe_experts(ctypes.byref(g), _ptr(slab), _table_ptr(table, n_experts),
+                                 n_experts, x.data_ptr(), inds.data_ptr(), weights.data_ptr(), n,
+                                 k, int(shared_slot), _ptr(shared_gate), out.data_ptr(),
+                                 ws.data_ptr(), ws.numel(), _stream()), "pmoe_moe_experts")
     return out
 
 
@@ -435,6 +449,9 @@ def combine(y: torch.Tensor, weights: torch.Tensor, shared_y=None, shared_logit=
     return out
 
 
+_STREAM_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
+
+
 def _stream_dtype(t, name, dtype=None):
     """The ABI's type of an fp32 or bf16 tensor (of ``dtype``, if given)."""
     if not isinstance(t, torch.Tensor) or t.dtype not in (torch.float32, torch.bfloat16):
@@ -452,18 +469,29 @@ def _like(t, ref, shape, name, dtype=None):
     _same_device(ref, t, name)
 
 
+def _bf16_rows(x):
+    """A new bf16 tensor like the contiguous x (the shorter way where x is bf16)."""
+    if x.dtype is torch.bfloat16:
+        return torch.empty_like(x)
+    return x.new_empty(x.shape, dtype=torch.bfloat16)
+
+
 def block_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
                unit_offset: bool = False) -> torch.Tensor:
     """h [N, D] bf16: the RMS norm of a residual stream x [N, D] (fp32 or
     bf16) with weight [D] (fp32 or bf16; 1 + weight with unit_offset), the
     input of a block (pmoe_block_norm)."""
-    xd, wd = _stream_dtype(x, "x"), _stream_dtype(weight, "weight")
+    try:
+        xd, wd = _STREAM_DTYPES[x.dtype], _STREAM_DTYPES[weight.dtype]
+    except (AttributeError, KeyError, TypeError):  # says which it is
+        xd, wd = _stream_dtype(x, "x"), _stream_dtype(weight, "weight")
     if not (x.dim() == 2 and x.is_cuda and x.is_contiguous()):
         _need(x, x.dtype, "x", 2)
     n, d = x.shape
-    if not _fits(weight, weight.dtype, (d,), x.get_device()):
+    if not (weight.shape == (d,) and weight.get_device() == x.get_device()
+            and weight.is_contiguous()):
         _like(weight, x, (d,), "weight")
-    h = x.new_empty((n, d), dtype=torch.bfloat16)
+    h = _bf16_rows(x)
     if n:
         check(lib().pmoe_block_norm(x.data_ptr(), xd, weight.data_ptr(), wd, n, d, eps,
                                     1 if unit_offset else 0, h.data_ptr(), _stream_of(x)),
@@ -487,7 +515,10 @@ def block_join(residual: torch.Tensor, y: torch.Tensor, weights=None, *, shared_
     [N, 1] per token or [N, D], by itself or its sigmoid.  ``out`` may be
     ``residual`` itself; it overlaps no other input."""
     j = _lib.Join()
-    j.stream_dtype = _stream_dtype(residual, "residual")
+    try:
+        j.stream_dtype = _STREAM_DTYPES[residual.dtype]
+    except (AttributeError, KeyError, TypeError):
+        j.stream_dtype = _stream_dtype(residual, "residual")
     if not (residual.dim() == 2 and residual.is_cuda and residual.is_contiguous()):
         _need(residual, residual.dtype, "residual", 2)
     n, d = residual.shape
@@ -513,12 +544,14 @@ def block_join(residual: torch.Tensor, y: torch.Tensor, weights=None, *, shared_
             raise ValueError("shared_logit must hold N values, beside shared_y")
     if post_weight is not None:
         j.weight_dtype = _stream_dtype(post_weight, "post_weight")
-        if not _fits(post_weight, post_weight.dtype, (d,), dev):
+        if not (post_weight.shape == (d,) and post_weight.get_device() == dev
+                and post_weight.is_contiguous()):
             _like(post_weight, residual, (d,), "post_weight")
     if next_weight is not None:
         j.weight_dtype = _stream_dtype(next_weight, "next_weight",
                                        None if post_weight is None else post_weight.dtype)
-        if not _fits(next_weight, next_weight.dtype, (d,), dev):
+        if not (next_weight.shape == (d,) and next_weight.get_device() == dev
+                and next_weight.is_contiguous()):
             _like(next_weight, residual, (d,), "next_weight")
     if gate is not None:
         j.gate_dtype = _stream_dtype(gate, "gate")
@@ -531,16 +564,20 @@ def block_join(residual: torch.Tensor, y: torch.Tensor, weights=None, *, shared_
             j.gate_kind = _lib.GATE_ELEMENT
         else:
             raise ValueError(f"gate: expected {(d,)}, {(n, 1)} or {(n, d)}, got {tuple(shape)}")
-        if not _fits(gate, gate.dtype, shape, dev):
+        if not (gate.get_device() == dev and gate.is_contiguous()):
             _like(gate, residual, shape, "gate")
-    j.gate_sigmoid = 1 if gate_sigmoid else 0
-    j.unit_offset = 1 if unit_offset else 0
+        if gate_sigmoid:
+            j.gate_sigmoid = 1
+    if unit_offset:
+        j.unit_offset = 1
     j.residual_scale, j.branch_scale, j.eps = residual_scale, branch_scale, eps
     if out is None:
         out = torch.empty_like(residual)
     elif not _fits(out, residual.dtype, (n, d), dev):
         _like(out, residual, (n, d), "out", residual.dtype)
-    h = residual.new_empty((n, d), dtype=bf16) if next_weight is not None else None
+    h = None
+    if next_weight is not None:  # (y is bf16 of that shape where it has no slots)
+        h = torch.empty_like(y) if weights is None else _bf16_rows(residual)
     if n:
         check(lib().pmoe_block_join(
             ctypes.byref(j), residual.data_ptr(), y.data_ptr(), _ptr(weights), _ptr(shared_y),
@@ -572,6 +609,9 @@ def moe_block(g: Geom, rc: RouteCfg, slab, table, gate_w, x, score_bias=None, lo
     n = x.shape[0]
     k = rc.top_k
     dev = x.device
+    if x.shape[1] != g.hidden or gate_w.shape[1] != g.hidden or gate_w.shape[0] < rc.n_experts:
+        raise ValueError(f"x must be [N, {g.hidden}] and gate_w [{rc.n_experts}, {g.hidden}], got "
+                         f"{tuple(x.shape)} and {tuple(gate_w.shape)}")
     if out is None:
         out = torch.empty((n, g.hidden), dtype=torch.bfloat16, device=dev)
     if inds is None:
@@ -580,7 +620,8 @@ def moe_block(g: Geom, rc: RouteCfg, slab, table, gate_w, x, score_bias=None, lo
         weights = torch.empty((n, k), dtype=torch.float32, device=dev)
     if ws is None:
         ws = moe_workspace(g, n, k, int(shared_slot >= 0), rc.n_experts, dev)
-    check(lib().pmoe_moe_block(ctypes.byref(g), ctypes.byref(rc), _ptr(slab), _table_ptr(table),
+    check(lib().pmoe_moe_block(ctypes.byref(g), ctypes.byref(rc), _ptr(slab),
+                               _table_ptr(table, rc.n_experts),
                                _ptr(gate_w), _ptr(score_bias), _ptr(logit_bias), _ptr(x), n,
                                int(shared_slot), _ptr(shared_gate), _ptr(out), _ptr(inds),
                                _ptr(weights), _ptr(ws), ws.numel(), _stream()), "pmoe_moe_block")

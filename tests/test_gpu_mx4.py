@@ -693,6 +693,27 @@ def test_large_calls_gate_and_zero_rows(n):
     assert (y.cpu()[gone].view(torch.int16) == 0).all()
 
 
+def test_calls_whose_arrays_do_not_fit_are_refused():
+    L = Layer(256, 128, 4)
+    x = tokens(np.random.default_rng(0), 3, 256)
+    i, w = torch.zeros(3, 2, dtype=torch.int32, device=DEV), torch.ones(3, 2, device=DEV)
+    a = (L.g, L.slab.buf, L.table, 4)
+    rc = K.route_cfg("softmax", 4, 2)
+    gate_w = torch.zeros(4, 256, device=DEV, dtype=torch.bfloat16)
+    for bad in (lambda: K.switch_glu(*a, x[:2], i), lambda: K.switch_glu(*a, x[:, :128].contiguous(), i),
+                lambda: K.switch_glu(*a, x.float(), i), lambda: K.switch_glu(*a, x, i.long()),
+                lambda: K.switch_glu(*a, x.cpu(), i), lambda: K.switch_glu(*a[:2], L.table[:3], 4, x, i),
+                lambda: K.moe_experts(*a, x[:2], i, w), lambda: K.moe_experts(*a, x, i, w[:2]),
+                lambda: K.moe_experts(*a, x, i, w[:, :1].contiguous()),
+                lambda: K.moe_experts(*a, x, i, w.t()), lambda: K.moe_experts(*a, x, i, w.half()),
+                lambda: K.moe_experts(*a, x, i, w, 3, gate_w[:1, :128].contiguous()),
+                lambda: K.moe_block(L.g, rc, L.slab.buf, L.table, gate_w[:3], x),
+                lambda: K.moe_block(L.g, rc, L.slab.buf, L.table, gate_w, x[:, :128].contiguous()),
+                lambda: K.moe_block(L.g, rc, L.slab.buf, L.table[:2], gate_w, x)):
+        with pytest.raises((TypeError, ValueError)):
+            bad()
+
+
 def test_empty_call():
     L = Layer(96, 64, 2)
     y = K.switch_glu(L.g, L.slab.buf, L.table, 2, torch.empty(0, 96, dtype=torch.bfloat16, device=DEV),
