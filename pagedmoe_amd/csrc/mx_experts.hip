@@ -1040,6 +1040,11 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void mx_tile_kernel(const MxArg
     }
   };
 
+  // Which part goes out with row tile i.  The down projection's activations follow
+  // each other and come sooner than its weights, which go first (16384 tokens 1218 ->
+  // 1180 us; gate/up gathers its activations, and loses 3% of 2048 tokens by it).
+  const auto turn = [](int i) { return DUAL ? i : i ^ 2; };
+
   const int rh = wave & 1, wq = wave >> 1;  // this wave's half of the rows, quarter of the weights
   f32x4 acc[8][4];
 #pragma unroll
@@ -1123,7 +1128,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void mx_tile_kernel(const MxArg
       // before this row tile's products
       if (i + 1 < NT) read(i + 1);
       __builtin_amdgcn_sched_barrier(0);
-      if (more) issue(ahead, buf ^ 1, block_ahead, i);
+      if (more) issue(ahead, buf ^ 1, block_ahead, turn(i));
       const uint4(&d)[3] = c[i & 1];
       const int sa = int(sa4[i]);
       const uint32_t b0[6] = {d[0].x, d[0].y, d[0].z, d[0].w, d[1].x, d[1].y};
@@ -1147,7 +1152,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void mx_tile_kernel(const MxArg
     }
     if (more) {
 #pragma unroll
-      for (int part = NT; part < 4; ++part) issue(ahead, buf ^ 1, block_ahead, part);
+      for (int i = NT; i < 4; ++i) issue(ahead, buf ^ 1, block_ahead, turn(i));
       ++ahead.s;
     }
     ++todo.s;
