@@ -19,7 +19,7 @@ namespace pmoe {
 
 namespace {
 
-constexpr int kChunk = 256;        // rows per block in the multi-block path
+constexpr int kChunk = kDispatchChunk;
 
 __global__ __launch_bounds__(1024) void dispatch_small_kernel(
     const IdSrc src, int rows, int n_experts, int32_t* __restrict__ order,
@@ -47,66 +47,12 @@ __global__ __launch_bounds__(kChunk) void dispatch_count_kernel(
     hist[size_t(blockIdx.x) * n_experts + e] = block_count<4>(s_wc, e);
 }
 
-// Phase 2 (one block): turn hist[b][e] into each block's base position per
-// expert and produce counts/offsets/active/tiles.  Thread e walks column e of
-// hist; its first kKeep entries are loaded in one round (all in flight) and
-// kept in registers for the second pass, so up to kKeep blocks (16,384 rows)
-// cost one round of loads instead of two passes of dependent rounds.
 __global__ __launch_bounds__(1024) void dispatch_scan_kernel(
     int32_t* __restrict__ hist, int n_blocks, int n_experts, int32_t* __restrict__ counts,
     int32_t* __restrict__ offsets, int32_t* __restrict__ active, int32_t* __restrict__ n_active,
     const TileSink ts) {
-  __shared__ int s_cnt[kMaxExperts];
-  __shared__ int s_off[kMaxExperts];
-  __shared__ int s_tmp[48];
-  constexpr int kKeep = 64;   // block histograms held in registers
-  constexpr int kBatch = 16;  // further block histograms read per round, all in flight
-  const int e = threadIdx.x;
-  int hk[kKeep];
-  if (e < n_experts) {
-    // clamped index: straight-line loads, no branch per entry (n_blocks >= 1),
-    // every load issued before the first is used
-#pragma unroll
-    for (int j = 0; j < kKeep; ++j)
-      hk[j] = hist[size_t(j < n_blocks ? j : n_blocks - 1) * n_experts + e];
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int j = 0; j < kKeep; ++j) hk[j] = j < n_blocks ? hk[j] : 0;
-    int run = 0;
-#pragma unroll
-    for (int j = 0; j < kKeep; ++j) run += hk[j];
-    for (int b0 = kKeep; b0 < n_blocks; b0 += kBatch) {
-      int h[kBatch];
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j)
-        h[j] = b0 + j < n_blocks ? hist[size_t(b0 + j) * n_experts + e] : 0;
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) run += h[j];
-    }
-    s_cnt[e] = run;
-  }
-  __syncthreads();
-  finish_scan(s_cnt, n_experts, counts, offsets, active, n_active, ts, s_off, s_tmp);
-  if (e < n_experts) {
-    // each block's base position per expert: expert offset + earlier blocks
-    int run = s_off[e];
-#pragma unroll
-    for (int j = 0; j < kKeep; ++j) {
-      if (j < n_blocks) hist[size_t(j) * n_experts + e] = run;
-      run += hk[j];
-    }
-    for (int b0 = kKeep; b0 < n_blocks; b0 += kBatch) {
-      int h[kBatch];
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j)
-        h[j] = b0 + j < n_blocks ? hist[size_t(b0 + j) * n_experts + e] : 0;
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        if (b0 + j < n_blocks) hist[size_t(b0 + j) * n_experts + e] = run;
-        run += h[j];
-      }
-    }
-  }
+  __shared__ ScanLds lds;
+  dispatch_scan(lds, hist, n_blocks, n_experts, counts, offsets, active, n_active, ts);
 }
 
 // Phase 3: scatter rows to their positions.
@@ -131,6 +77,22 @@ size_t dispatch_workspace(int rows, int n_experts) {
   if (rows <= kSmallRows) return 256;
   const size_t blocks = (rows + kChunk - 1) / kChunk;
   return ((blocks * n_experts + rows) * sizeof(int32_t) + 255) / 256 * 256;
+}
+
+int dispatch_count(const IdSrc& src, int rows, int n_ids, int32_t* hist, int32_t* rank,
+                   hipStream_t st) {
+  const int blocks = (rows + kChunk - 1) / kChunk;
+  dispatch_count_kernel<<<blocks, kChunk, 0, st>>>(src, rows, n_ids, hist, rank);
+  PMOE_LAUNCH_CHECK("dispatch_count_kernel");
+  return PMOE_OK;
+}
+
+int dispatch_scatter(const IdSrc& src, int rows, int n_ids, const int32_t* hist,
+                     const int32_t* rank, int32_t* order, int32_t* inv, hipStream_t st) {
+  const int blocks = (rows + kChunk - 1) / kChunk;
+  dispatch_scatter_kernel<<<blocks, kChunk, 0, st>>>(src, rows, n_ids, hist, rank, order, inv);
+  PMOE_LAUNCH_CHECK("dispatch_scatter_kernel");
+  return PMOE_OK;
 }
 
 // Internal entry: also builds the prefill tile list when tile_m > 0 (slots
@@ -160,14 +122,11 @@ int dispatch_ext(const int32_t* inds, int rows, int k_routed, int kk, int n_ids,
   const int blocks = (rows + kChunk - 1) / kChunk;
   int32_t* hist = static_cast<int32_t*>(ws);
   int32_t* rank = hist + size_t(blocks) * n_ids;
-  dispatch_count_kernel<<<blocks, kChunk, 0, st>>>(src, rows, n_ids, hist, rank);
-  PMOE_LAUNCH_CHECK("dispatch_count_kernel");
+  if (int rc = dispatch_count(src, rows, n_ids, hist, rank, st)) return rc;
   dispatch_scan_kernel<<<1, 1024, 0, st>>>(hist, blocks, n_ids, counts, offsets, active,
                                            n_active, ts);
   PMOE_LAUNCH_CHECK("dispatch_scan_kernel");
-  dispatch_scatter_kernel<<<blocks, kChunk, 0, st>>>(src, rows, n_ids, hist, rank, order, inv);
-  PMOE_LAUNCH_CHECK("dispatch_scatter_kernel");
-  return PMOE_OK;
+  return dispatch_scatter(src, rows, n_ids, hist, rank, order, inv, st);
 }
 
 }  // namespace pmoe

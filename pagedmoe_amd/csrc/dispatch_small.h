@@ -1,5 +1,5 @@
-// One-block dispatch, shared by the dispatch launch (dispatch.hip) and by launches
-// that dispatch beside other work.
+// The dispatch's one-block steps, shared by its own launches (dispatch.hip) and by
+// launches that do them beside other work.
 #pragma once
 
 #include "pmoe_internal.h"
@@ -8,6 +8,7 @@
 namespace pmoe {
 
 constexpr int kSmallRows = 1024;   // rows that one block dispatches
+constexpr int kDispatchChunk = 256;  // rows per block in the multi-block path
 constexpr int kMaxExperts = 1024;
 
 // Source of flat row ids: row r = n*kk + c reads inds[n*k_routed + c] for
@@ -227,5 +228,78 @@ __device__ __forceinline__ void dispatch_small(DispatchLds& l, const IdSrc& src,
     inv[tid] = -1;
   }
 }
+
+// Phase 2 (one block): turn hist[b][e] into each block's base position per
+// expert and produce counts/offsets/active/tiles.  Thread e walks column e of
+// hist; its first kKeep entries are loaded in one round (all in flight) and
+// kept in registers for the second pass, so up to kKeep blocks (16,384 rows)
+// cost one round of loads instead of two passes of dependent rounds.
+struct ScanLds {
+  int cnt[kMaxExperts];
+  int off[kMaxExperts];
+  int tmp[48];
+};
+
+__device__ __forceinline__ void dispatch_scan(ScanLds& l, int32_t* __restrict__ hist, int n_blocks,
+                                              int n_experts, int32_t* __restrict__ counts,
+                                              int32_t* __restrict__ offsets,
+                                              int32_t* __restrict__ active,
+                                              int32_t* __restrict__ n_active, const TileSink& ts) {
+  constexpr int kKeep = 64;   // block histograms held in registers
+  constexpr int kBatch = 16;  // further block histograms read per round, all in flight
+  const int e = threadIdx.x;
+  int hk[kKeep];
+  if (e < n_experts) {
+    // clamped index: straight-line loads, no branch per entry (n_blocks >= 1),
+    // every load issued before the first is used
+#pragma unroll
+    for (int j = 0; j < kKeep; ++j)
+      hk[j] = hist[size_t(j < n_blocks ? j : n_blocks - 1) * n_experts + e];
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < kKeep; ++j) hk[j] = j < n_blocks ? hk[j] : 0;
+    int run = 0;
+#pragma unroll
+    for (int j = 0; j < kKeep; ++j) run += hk[j];
+    for (int b0 = kKeep; b0 < n_blocks; b0 += kBatch) {
+      int h[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        h[j] = b0 + j < n_blocks ? hist[size_t(b0 + j) * n_experts + e] : 0;
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) run += h[j];
+    }
+    l.cnt[e] = run;
+  }
+  __syncthreads();
+  finish_scan(l.cnt, n_experts, counts, offsets, active, n_active, ts, l.off, l.tmp);
+  if (e < n_experts) {
+    // each block's base position per expert: expert offset + earlier blocks
+    int run = l.off[e];
+#pragma unroll
+    for (int j = 0; j < kKeep; ++j) {
+      if (j < n_blocks) hist[size_t(j) * n_experts + e] = run;
+      run += hk[j];
+    }
+    for (int b0 = kKeep; b0 < n_blocks; b0 += kBatch) {
+      int h[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        h[j] = b0 + j < n_blocks ? hist[size_t(b0 + j) * n_experts + e] : 0;
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        if (b0 + j < n_blocks) hist[size_t(b0 + j) * n_experts + e] = run;
+        run += h[j];
+      }
+    }
+  }
+}
+
+// The launches before and after the scan (dispatch.hip): hist [blocks of
+// kDispatchChunk rows, n_ids], rank [rows].
+int dispatch_count(const IdSrc& src, int rows, int n_ids, int32_t* hist, int32_t* rank,
+                   hipStream_t st);
+int dispatch_scatter(const IdSrc& src, int rows, int n_ids, const int32_t* hist,
+                     const int32_t* rank, int32_t* order, int32_t* inv, hipStream_t st);
 
 }  // namespace pmoe

@@ -185,7 +185,7 @@ struct MxSplit {
 // A token by 256 threads, a lane a group: its pieces, scales and the mask of the
 // 128-wide steps that hold a third piece (16 bits a wave), the shared expert's gate
 // logit, the zero rows of ids that are dropped.  s_sum: 4 floats of the token's.
-// 16384 x 4096: 134 MB in, 280 MB out, 48 us.  Splitting in the products instead
+// 16384 x 4096: 134 MB in, 280 MB out, 64 us beside the dispatch's scan.  Splitting in the products instead
 // would repeat these ~20 operations a value for every block of features.
 __device__ __forceinline__ void split_token(const MxSplit& a, int token, int g, float* s_sum) {
   bool peak = false;
@@ -245,17 +245,13 @@ __device__ __forceinline__ void split_token(const MxSplit& a, int token, int g, 
   }
 }
 
-__global__ __launch_bounds__(256) void mx_split_kernel(const MxSplit a) {
-  __shared__ float s_sum[4];
-  split_token(a, blockIdx.x, threadIdx.x, s_sum);
-}
-
 // The dispatch of a small call beside its split: block 0 dispatches, the others
 // take four tokens each.  5 us for 24 rows, 7 for 800: the dispatching block's
 // barriers, under which the split hides (two launches took 4 us more).
 struct MxDispatch {
   IdSrc src;
   int rows, n_ids;
+  int32_t* hist;  // large calls: the counts of each kDispatchChunk rows
   int32_t *order, *counts, *offsets, *inv, *active, *n_active;
   TileSink tiles;
 };
@@ -265,6 +261,21 @@ __global__ __launch_bounds__(1024) void mx_prepare_kernel(const MxSplit a, const
   if (blockIdx.x == 0) {
     dispatch_small(lds, d.src, d.rows, d.n_ids, d.order, d.counts, d.offsets, d.inv, d.active,
                    d.n_active, d.tiles);
+    return;
+  }
+  const int quarter = threadIdx.x >> 8;
+  split_token(a, (blockIdx.x - 1) * 4 + quarter, threadIdx.x & 255,
+              reinterpret_cast<float*>(lds.tmp) + 4 * quarter);
+}
+
+// The same of a large call, between the dispatch's count and its scatter: block 0
+// scans (4096 tokens x 10 of 2048, the whole call 456 -> 443 us against two launches;
+// 16384 x 8 of 4096: 48 + 39 -> 64).
+__global__ __launch_bounds__(1024) void mx_scan_split_kernel(const MxSplit a, const MxDispatch d) {
+  __shared__ ScanLds lds;
+  if (blockIdx.x == 0) {
+    dispatch_scan(lds, d.hist, (d.rows + kDispatchChunk - 1) / kDispatchChunk, d.n_ids, d.counts,
+                  d.offsets, d.active, d.n_active, d.tiles);
     return;
   }
   const int quarter = threadIdx.x >> 8;
@@ -1361,24 +1372,33 @@ int mx_experts(const MxPlan& p, hipStream_t st) {
   sp.shared_gate = p.shared_gate, sp.shared_logit = p.shared_logit;
   sp.ids = p.ids, sp.k = p.k, sp.n_experts = p.n_experts;
   sp.y = p.yscale ? nullptr : p.y;
+  MxDispatch d{};
+  d.src = IdSrc{p.ids, p.k, p.kk, p.n_experts};
+  d.rows = rows, d.n_ids = n_ids;
+  d.order = p.order, d.counts = p.counts, d.offsets = p.offsets, d.inv = p.inv;
+  d.active = p.active, d.n_active = p.n_active;
+  d.tiles = TileSink{p.tiles, p.n_tiles, p.tile_rows, p.table, p.n_experts, p.shared_slot};
+  const int split_blocks = (p.n + 3) / 4;
   if (rows <= kSmallRows) {
-    MxDispatch d{};
-    d.src = IdSrc{p.ids, p.k, p.kk, p.n_experts};
-    d.rows = rows, d.n_ids = n_ids;
-    d.order = p.order, d.counts = p.counts, d.offsets = p.offsets, d.inv = p.inv;
-    d.active = p.active, d.n_active = p.n_active;
-    d.tiles = TileSink{p.tiles, p.n_tiles, p.tile_rows, p.table, p.n_experts, p.shared_slot};
     ProfScope prof_scope(K_MX_SPLIT, st);
-    mx_prepare_kernel<<<1 + (p.n + 3) / 4, 1024, 0, st>>>(sp, d);
+    mx_prepare_kernel<<<1 + split_blocks, 1024, 0, st>>>(sp, d);
     PMOE_LAUNCH_CHECK("mx_prepare_kernel");
   } else {
-    if (int rc = dispatch_ext(p.ids, rows, p.k, p.kk, n_ids, p.order, p.counts, p.offsets, p.inv,
-                              p.active, p.n_active, p.tile_rows, p.tiles, p.n_tiles, p.table,
-                              p.shared_slot, p.dws, p.dws_bytes, st))
-      return rc;
-    ProfScope prof_scope(K_MX_SPLIT, st);
-    mx_split_kernel<<<p.n, 256, 0, st>>>(sp);
-    PMOE_LAUNCH_CHECK("mx_split_kernel");
+    PMOE_REQUIRE(p.dws != nullptr && p.dws_bytes >= dispatch_workspace(rows, n_ids),
+                 "dispatch: workspace too small");
+    d.hist = static_cast<int32_t*>(p.dws);
+    int32_t* rank = d.hist + size_t((rows + kDispatchChunk - 1) / kDispatchChunk) * n_ids;
+    {
+      ProfScope prof_scope(K_DISPATCH, st);
+      if (int rc = dispatch_count(d.src, rows, n_ids, d.hist, rank, st)) return rc;
+    }
+    {
+      ProfScope prof_scope(K_MX_SPLIT, st);
+      mx_scan_split_kernel<<<1 + split_blocks, 1024, 0, st>>>(sp, d);
+      PMOE_LAUNCH_CHECK("mx_scan_split_kernel");
+    }
+    ProfScope prof_scope(K_DISPATCH, st);
+    if (int rc = dispatch_scatter(d.src, rows, n_ids, d.hist, rank, p.order, p.inv, st)) return rc;
   }
   const bool once = rows <= int64_t(kFewRows) * p.n_experts;
   MxArgs a{};
