@@ -466,6 +466,82 @@ def test_custom_slot_layout_and_streams():
     assert torch.equal(y, z)
 
 
+@pytest.mark.parametrize("gap", [1, 2, 4, 8])
+@pytest.mark.parametrize("n,pin", [(1, "0"), (20, "0"), (300, "0"), (300, "1")])
+def test_scales_anywhere(monkeypatch, n, pin, gap):
+    """Scales on no word, on 4 and on 8 bytes give the outputs of scales on 256: the
+    forms that fetch them by words and by 16 bytes step aside."""
+    monkeypatch.setenv("PMOE_MX_TILE", pin)
+    rng = np.random.default_rng(gap)
+    hidden, inter = 1024, 512
+    L = Layer(hidden, inter, 3)
+    g = _lib.geom(hidden, inter, 4, 32)
+    specs = component_specs(L.g)
+    comps = ((0, "gate_proj.weight"), (1, "gate_proj.scales"), (3, "up_proj.weight"),
+             (4, "up_proj.scales"), (6, "down_proj.weight"), (7, "down_proj.scales"))
+    at = 0
+    for c, name in comps:
+        at = (at + 15) // 16 * 16 + (gap if name.endswith("scales") else 0)
+        g.off[c] = at
+        at += g.nbytes[c]
+    g.expert_bytes = (at + 15) // 16 * 16
+    buf = torch.full((3 * g.expert_bytes,), 0xFF, dtype=torch.uint8, device=DEV)
+    for e in range(3):
+        for c, name in comps:
+            dst = e * g.expert_bytes + g.off[c]
+            buf[dst:dst + specs[name][2]] = L.slab.dest(name, e)
+    x = tokens(rng, n, hidden)
+    inds = torch.from_numpy(rng.integers(0, 3, (n, 2)).astype(np.int32)).to(DEV)
+    want = K.switch_glu(L.g, L.slab.buf, L.table, 3, x, inds)
+    assert torch.equal(want, K.switch_glu(g, buf, L.table, 3, x, inds))
+
+
+def test_slots_past_32_bits():
+    """A slot that begins past 4 GiB of the slab gives a near slot's outputs."""
+    rng = np.random.default_rng(0)
+    L = Layer(1024, 512, 2)
+    size = int(L.g.expert_bytes)
+    far = (5 << 30) // size
+    buf = torch.empty((far + 1) * size, dtype=torch.uint8, device=DEV)
+    buf[far * size:] = L.slab.buf[:size]
+    buf[(far - 3) * size:(far - 2) * size] = L.slab.buf[size:2 * size]
+    table = torch.tensor([far, far - 3], dtype=torch.int32, device=DEV)
+    near = torch.tensor([0, 1], dtype=torch.int32, device=DEV)
+    for n in (1, 5, 400):
+        x = tokens(rng, n, 1024)
+        inds = torch.from_numpy(np.tile(np.array([[1, 0]], np.int32), (n, 1))).to(DEV)
+        assert torch.equal(K.switch_glu(L.g, buf, table, 2, x, inds),
+                           K.switch_glu(L.g, L.slab.buf, near, 2, x, inds))
+
+
+@pytest.mark.parametrize("pin", ["0", "1"])
+def test_rows_past_32_bits(monkeypatch, pin):
+    """Slot outputs and seam rows of more than 4 GiB: the last rows are those of a
+    call of their own."""
+    import ctypes
+    monkeypatch.setenv("PMOE_MX_TILE", pin)
+    hidden, inter, n, k = 8192, 64 if pin == "0" else 128, 36000, 8
+    L = Layer(hidden, inter, 3)
+    g = torch.Generator(device=DEV).manual_seed(0)
+    x = torch.randn(n, hidden, device=DEV, generator=g).to(torch.bfloat16)
+    inds = torch.randint(-1, 3, (n, k), device=DEV, generator=g, dtype=torch.int32)
+    w = torch.rand(n, k, device=DEV, generator=g)
+    ws = K.moe_workspace(L.g, n, k, 0, 3, x.device, fresh=True)
+    out = torch.empty_like(x)
+    y = torch.empty(n, k, hidden, device=DEV, dtype=torch.bfloat16)
+    lib, p = _lib.lib(), ctypes.byref(L.g)
+    args = (p, L.slab.buf.data_ptr(), L.table.data_ptr(), 3, x.data_ptr(), inds.data_ptr())
+    _lib.check(lib.pmoe_moe_experts(*args, w.data_ptr(), n, k, -1, None, out.data_ptr(),
+                                    ws.data_ptr(), ws.numel(), K._stream()))
+    _lib.check(lib.pmoe_switch_glu(*args, n, k, y.data_ptr(), ws.data_ptr(), ws.numel(),
+                                   K._stream()))
+    for r in (slice(0, 200), slice(n - 200, n)):
+        i = inds[r].contiguous()
+        assert torch.equal(y[r], K.switch_glu(L.g, L.slab.buf, L.table, 3, x[r].contiguous(), i))
+        assert torch.equal(out[r], K.moe_experts(L.g, L.slab.buf, L.table, 3, x[r].contiguous(), i,
+                                                 w[r].contiguous()))
+
+
 @pytest.mark.parametrize("n", [1, 6, 200])
 def test_captured_and_replayed(n):
     """A captured call gives the eager bits on every replay, with other work on

@@ -179,6 +179,21 @@ def test_rows_do_not_depend_on_their_number(d):
         assert torch.equal(nh[r0:r1], K.block_norm(part["residual"], a["next_weight"]))
 
 
+@pytest.mark.parametrize("d", [8192, 8191])
+def test_rows_past_32_bits(d):
+    """More than 2^32 elements: the last rows are those of a call of their own."""
+    n = 2 ** 32 // d + 100
+    x = torch.empty(n, d, device=DEV, dtype=torch.bfloat16)
+    x[-50:] = torch.randn(50, d, device=DEV, generator=gen(1)).to(torch.bfloat16)
+    x[:-50] = 1
+    w = torch.randn(d, device=DEV, generator=gen(2))
+    tail = x[-50:].clone()
+    assert torch.equal(K.block_norm(x, w)[-50:], K.block_norm(tail, w))
+    out, h = K.block_join(x, x, gate=w, next_weight=w)
+    o, hh = K.block_join(tail, tail, gate=w, next_weight=w)
+    assert torch.equal(out[-50:], o) and torch.equal(h[-50:], hh)
+
+
 @pytest.mark.parametrize("stream", [torch.bfloat16, torch.float32])
 def test_past_the_caches(stream):
     """Results of more than 64 MiB, in place too: the rows that shorter calls give."""
