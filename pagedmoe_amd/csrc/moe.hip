@@ -53,7 +53,7 @@ struct MoeWs {
   uint8_t *xpair = nullptr, *xthird = nullptr, *xscale = nullptr;
   uint16_t* xsteps = nullptr;
   uint8_t *hpair = nullptr, *hscale = nullptr;
-  float* h32 = nullptr;       // a single token's intermediate
+  float* h32 = nullptr;       // single tokens' intermediate
   uint8_t* yscale = nullptr;  // of the slot outputs that the combine reads
 };
 
@@ -98,7 +98,9 @@ size_t carve(const pmoe_geom* g, int n, int k, int shared, int n_experts, void* 
     t.hpair = c.take<uint8_t>(hs * kMxStepPair);
     t.hscale = c.take<uint8_t>(rows * mx_scale_row(g->inter));
     t.y = reinterpret_cast<float*>(c.take<uint16_t>(rows * g->hidden));
-    t.h32 = n == 1 ? c.take<float>(rows * g->inter) : nullptr;
+    // (also in longer calls' workspaces, which serve shorter calls)
+    const int one = std::min(n, mx_one_tokens(g, k, shared ? 1 : 0, n_experts, true));
+    t.h32 = c.take<float>(size_t(one) * kk * g->inter);
     t.yscale = c.take<uint8_t>(rows * (g->hidden / kMxGroup));
   } else {
     t.h = c.take<uint16_t>(rows * g->inter);
@@ -560,14 +562,14 @@ int experts_and_combine(const pmoe_geom* g, const uint8_t* slab, const int32_t* 
   const int kk = k + shared;
   if (is_mx(g)) {
     const uint16_t* gate = shared ? shared_gate : nullptr;
-    if (n > 1 || !mx_one_covers(kk)) {
+    if (!mx_one_wanted(g, n, k, shared, n_experts, true)) {
       if (int rc = run_mx(g, slab, table, n_experts, shared_slot, gate, x, inds, n, k, kk, w,
                           nullptr, st))
         return rc;
       return mx_combine(reinterpret_cast<const uint16_t*>(w.y), w.yscale, wts, w.inv,
                         gate ? w.shared_logit : nullptr, n, k, kk, g->hidden, out, st);
     }
-    return mx_one(g, slab, table, n_experts, x, inds, wts, k, shared_slot, gate,
+    return mx_one(g, slab, table, n_experts, x, inds, wts, n, k, shared_slot, gate,
                   w.shared_logit, w.order, w.h32, out, st);
   }
   if (n == 1 && k == kXcdCount && !(shared && shared_gate)) {
@@ -677,9 +679,9 @@ extern "C" int pmoe_switch_glu(const pmoe_geom* g, const void* slab, const int32
   MoeWs w;
   pmoe::carve(g, n, k, 0, n_experts, ws, &w);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (n == 1 && pmoe::is_mx(g) && pmoe::mx_one_covers(k))
+  if (pmoe::is_mx(g) && pmoe::mx_one_wanted(g, n, k, 0, n_experts, false))
     return pmoe::mx_one(g, static_cast<const uint8_t*>(slab), table, n_experts,
-                        static_cast<const uint16_t*>(x), inds, nullptr, k, -1, nullptr, nullptr,
+                        static_cast<const uint16_t*>(x), inds, nullptr, n, k, -1, nullptr, nullptr,
                         w.order, w.h32, static_cast<uint16_t*>(y), st);
   if (pmoe::is_mx(g))
     return pmoe::run_mx(g, static_cast<const uint8_t*>(slab), table, n_experts, -1, nullptr,

@@ -62,11 +62,13 @@ int mx_tile_rows(const pmoe_geom* g, int n, int kk, int n_experts);
 int mx_min_tile_rows();
 // Dispatch, split, gate/up, down; rows whose expert is not resident come out zero.
 int mx_experts(const MxPlan& p, hipStream_t st);
-// One token in two launches, without a dispatch: out bf16 [hidden] combined (wts
-// given) or [k, hidden].  slots [k + 1], h fp32 [k + 1, inter]: scratch.
-bool mx_one_covers(int kk);
+// Tokens one by one in two launches, without a dispatch: out bf16 [n, hidden]
+// combined (wts given) or [n, k, hidden].  slots [n, k + 1], h fp32 [n, k + 1, inter]:
+// scratch.  mx_one_tokens: the most tokens that go this way (the scratch's size).
+int mx_one_tokens(const pmoe_geom* g, int k, int shared, int n_experts, bool combined);
+bool mx_one_wanted(const pmoe_geom* g, int n, int k, int shared, int n_experts, bool combined);
 int mx_one(const pmoe_geom* g, const uint8_t* slab, const int32_t* table, int n_experts,
-           const uint16_t* x, const int32_t* ids, const float* wts, int k, int shared_slot,
+           const uint16_t* x, const int32_t* ids, const float* wts, int n, int k, int shared_slot,
            const uint16_t* shared_gate, float* shared_logit, int32_t* slots, float* h,
            uint16_t* out, hipStream_t st);
 // out[n] = sum over columns in order of weight * y (+ the shared column's).

@@ -9,17 +9,18 @@
 // a value stands out; the sums are fp32.
 //
 // Three forms, by the rows of the call:
-//   one token     two launches without a dispatch: gate/up from x itself, and the
-//                 down projection with the columns' weighted sum inside
+//   few tokens,   one by one, two launches without a dispatch: gate/up from x itself,
+//   small experts and the down projection with the columns' weighted sum inside
 //   few rows an   dispatch and activation pieces in one launch (mx_prepare_kernel),
 //   expert        tiles of 16 rows bound by the weights' stream, a combine
 //   many          tiles of 128 rows bound by the matrix instructions and the loads
 //                 beside them
-// The line between the last two stands at mx_tile_rows.
+// The lines between them stand at mx_one_tokens and mx_tile_rows.
 //
 // An activation that is infinite or NaN, or an intermediate that leaves fp32,
 // makes the outputs of its row NaN.
 #include <hip/hip_fp16.h>
+#include <math.h>
 #include <stdlib.h>
 
 #include <algorithm>
@@ -545,27 +546,41 @@ int launch_stream(const MxArgs& a, int max_tiles, bool once, bool whole, hipStre
   return PMOE_OK;
 }
 
-// ---------------------------------------------------------------- one token
+// ---------------------------------------------------------------- single tokens
 
 constexpr int kOneCols = 16;   // features a block
 constexpr int kOneBatch = 3;   // (column, stretch) items of the down projection in flight a wave
 
+// Every token by itself (blockIdx.z), its experts' weights read for it alone.
 struct MxOne {
   const uint8_t* slab;
   int64_t expert_bytes;
   const int32_t* table;
   int n_experts;
-  const int32_t* ids;   // [k]
-  const float* wts;     // [k]
+  const int32_t* ids;   // [n, k]
+  const float* wts;     // [n, k], or null: uncombined
   int k, kk, shared_slot;
   const uint16_t* shared_gate;  // or null
-  float* shared_logit;
-  int32_t* slots;       // [kk], found by the first launch for the second
+  float* shared_logit;  // [n]
+  int32_t* slots;       // [n, kk], found by the first launch for the second
   int64_t w0, s0, w1, s1, wd, sd;
-  const uint16_t* x;
+  const uint16_t* x;    // [n, hidden]
   int hidden, inter;
-  float* h;             // fp32 [kk, inter]
-  uint16_t* out;        // bf16: [hidden], or [kk, hidden] uncombined
+  float* h;             // fp32 [n, kk, inter]
+  uint16_t* out;        // bf16: [n, hidden], or [n, kk, hidden] uncombined
+
+  // the same with the arrays of one token
+  __device__ __forceinline__ MxOne of(int token) const {
+    MxOne a = *this;
+    a.ids += size_t(token) * k;
+    if (wts) a.wts += size_t(token) * k;
+    if (shared_logit) a.shared_logit += token;
+    a.slots += size_t(token) * kk;
+    a.x += size_t(token) * hidden;
+    a.h += size_t(token) * kk * inter;
+    a.out += size_t(token) * (wts ? 1 : kk) * hidden;
+    return a;
+  }
 };
 
 // Slot of column c, -1 where nothing is held.
@@ -639,9 +654,10 @@ __device__ __forceinline__ void one_mma(f32x4& acc, const uint8_t* w, const uint
 // 53 MB in 13.0 us, 4.1 TB/s: the two lookups, then two rounds of loads a wave (16
 // features a block were slower).
 template <bool WHOLE>
-__global__ __launch_bounds__(64 * kMaxWaves, 4) void mx_one_gateup_kernel(const MxOne a,
+__global__ __launch_bounds__(64 * kMaxWaves, 4) void mx_one_gateup_kernel(const MxOne all,
                                                                           int wave_lds) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t dyn[];
+  const MxOne a = all.of(blockIdx.z);
   constexpr int NF = 4, kCols = kStreamRows / 2;
   const int c = blockIdx.y, fb = blockIdx.x;
   const int waves = blockDim.x >> 6;
@@ -789,8 +805,10 @@ __global__ __launch_bounds__(64 * kMaxWaves, 4) void mx_one_gateup_kernel(const 
 // columns: 27 MB in 8.9 us, every load of a block in flight at once; what is left is
 // the launch, the slots' lookup and the sum at the end.
 template <bool MIX, bool WHOLE>
-__global__ __launch_bounds__(64 * kMaxWaves, 2) void mx_one_down_kernel(const MxOne a, int batch) {
+__global__ __launch_bounds__(64 * kMaxWaves, 2) void mx_one_down_kernel(const MxOne all,
+                                                                        int batch) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t dyn[];
+  const MxOne a = all.of(blockIdx.z);
   const int f0 = blockIdx.x * kOneCols;
   const int waves = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1315,6 +1333,12 @@ bool mx_aligned(const pmoe_geom* g) {
   return true;
 }
 
+// PMOE_MX_TILE=0 / 1 pins tiles of 16 / 128 rows (read per call).
+int mx_pinned_rows() {
+  const char* v = getenv("PMOE_MX_TILE");
+  return !v ? 0 : v[0] == '0' ? kFewRows : v[0] == '1' ? kTileRows : 0;
+}
+
 }  // namespace
 
 // Rows of a tile: 16 (streamed tiles, which read an expert's weights again for
@@ -1332,12 +1356,10 @@ bool mx_aligned(const pmoe_geom* g) {
 //   4128x1568, 128 experts  14: 535 / 644, 20: 604 / 657, 62: 1372 / 720
 //   2880x2880, 32 experts   12: 162 / 194, 19: 197 / 197
 //   1056x480, 32 experts    50: 43 / 44, 100: 68 / 47
-// PMOE_MX_TILE=0 / 1 pins 16 / 128 (read per call).
 int mx_tile_rows(const pmoe_geom* g, int n, int kk, int n_experts) {
   // the tokens' pieces within the large tiles' 32-bit offsets
   if (int64_t(n) * mx_steps(g->hidden) * kMxStepPair >= int64_t(1) << 32) return kFewRows;
-  const char* v = getenv("PMOE_MX_TILE");
-  if (v && (v[0] == '0' || v[0] == '1')) return v[0] == '1' ? kTileRows : kFewRows;
+  if (const int pinned = mx_pinned_rows()) return pinned;
   const int64_t rows = int64_t(n) * kk;
   const int64_t blocks =
       (n_experts + rows / kTileRows) * ((g->inter + kTileCols / 2 - 1) / (kTileCols / 2));
@@ -1431,12 +1453,41 @@ int mx_experts(const MxPlan& p, hipStream_t st) {
                : launch_stream<false, false>(a, p.max_tiles, once, whole, st);
 }
 
-// One token: two launches, no dispatch; out bf16 [hidden] combined (wts given), or
-// [kk, hidden].  Up to 64 columns: a lane looks one up.
-bool mx_one_covers(int kk) { return kk <= 64; }
+// The most tokens that go one by one (0: none may), in two launches instead of a
+// dispatch, the tiles' two and a combine.  What that saves, some 7 us and the combine,
+// pays for the weights that several of the tokens read (by expectation over
+// independent ids, and the shared expert's), and for a stream that is a tenth slower
+// than the tiles'.  us, tiles / one by one:
+//   1024x512 32 experts, 4 columns    8 tokens 19.0 / 11.8, 16: 20.2 / 14.4, 32: 22.1 / 22.4
+//   2048x512 512 experts, 10 + shared 2: 23.9 / 15.7, 4: 31.2 / 21.1, 8: 43.8 / 41.1
+//     seam, 10                        2: 19.3 / 14.2, 8: 36.6 / 35.7, 12: 46.6 / 49.0
+//   4096x1536 128 experts, 8          2: 43.8 / 39.2, 3: 56.5 / 56.6, 4: 66.6 / 70.6
+//     seam                            2: 40.2 / 38.5, 3: 53.3 / 53.8
+//   7168x2048 384 experts, 8 + shared 2: 91.7 / 94.0; seam, 8: 79.1 / 80.2
+// Up to 64 columns: a lane looks one up.
+int mx_one_tokens(const pmoe_geom* g, int k, int shared, int n_experts, bool combined) {
+  if (k + shared > 64) return 0;
+  const double bytes = double(g->hidden) * g->inter / kMxGroup * 17 * 3;
+  const double most = double((combined ? 36 : 24) << 20) / bytes;  // in experts
+  const double absent = pow(1.0 - 1.0 / n_experts, k);  // an expert of one token's
+  double none = absent;
+  int n = 1;
+  for (; n < 64; ++n) {  // would n + 1 do?
+    none *= absent;
+    const double repeated =
+        double(n + 1) * k - n_experts * (1.0 - none) + double(shared) * n;
+    if (repeated + 0.1 * (n + 1) * (k + shared) > most) break;
+  }
+  return n;
+}
+
+bool mx_one_wanted(const pmoe_geom* g, int n, int k, int shared, int n_experts, bool combined) {
+  if (n > 1 && mx_pinned_rows()) return false;
+  return n <= mx_one_tokens(g, k, shared, n_experts, combined);
+}
 
 int mx_one(const pmoe_geom* g, const uint8_t* slab, const int32_t* table, int n_experts,
-           const uint16_t* x, const int32_t* ids, const float* wts, int k, int shared_slot,
+           const uint16_t* x, const int32_t* ids, const float* wts, int n, int k, int shared_slot,
            const uint16_t* shared_gate, float* shared_logit, int32_t* slots, float* h,
            uint16_t* out, hipStream_t st) {
   MxOne a{};
@@ -1468,7 +1519,7 @@ int mx_one(const pmoe_geom* g, const uint8_t* slab, const int32_t* table, int n_
     const int wave_lds = (kStreamWave + rounds * 8 * (64 + 1) + 255) / 256 * 256;
     ProfScope prof_scope(K_MX_GATEUP, st);
     const auto go = [&](auto kernel) {
-      kernel<<<dim3(a.inter / (kStreamRows / 2), a.kk), 64 * waves, waves * wave_lds, st>>>(
+      kernel<<<dim3(a.inter / (kStreamRows / 2), a.kk, n), 64 * waves, waves * wave_lds, st>>>(
           a, wave_lds);
     };
     go(whole ? mx_one_gateup_kernel<true> : mx_one_gateup_kernel<false>);
@@ -1481,7 +1532,7 @@ int mx_one(const pmoe_geom* g, const uint8_t* slab, const int32_t* table, int n_
   const size_t lds = size_t(waves) * batch * kOneItem;
   ProfScope prof_scope(K_MX_DOWN, st);
   const auto go = [&](auto kernel) {
-    kernel<<<dim3(a.hidden / kOneCols, wts ? 1 : a.kk), 64 * waves, lds, st>>>(a, batch);
+    kernel<<<dim3(a.hidden / kOneCols, wts ? 1 : a.kk, n), 64 * waves, lds, st>>>(a, batch);
   };
   if (wts)
     go(whole ? mx_one_down_kernel<true, true> : mx_one_down_kernel<true, false>);

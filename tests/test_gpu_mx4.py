@@ -466,6 +466,39 @@ def test_custom_slot_layout_and_streams():
     assert torch.equal(y, z)
 
 
+@pytest.mark.parametrize("hidden,inter,experts,k", [
+    (256, 128, 6, 4), (96, 160, 5, 3), (1024, 512, 32, 4), (512, 256, 2, 2)])
+@pytest.mark.parametrize("n", [2, 7, 16, 63, 64, 65])
+def test_tokens_one_by_one(n, hidden, inter, experts, k):
+    """Few tokens of small experts: combined with a gated shared expert, dropped and
+    repeated ids and an absent expert; each token's bits are those of its own call."""
+    rng = np.random.default_rng(n * hidden)
+    L = Layer(hidden, inter, experts, 1, perm=True)
+    table = L.table.clone()
+    table[0] = -1
+    x = tokens(rng, n, hidden)
+    inds = rng.integers(-1, experts + 1, (n, k)).astype(np.int32)
+    w = rng.random((n, k)).astype(np.float32)
+    gate = bf16(rng.standard_normal((1, hidden)) * 0.05)
+    t, wt = torch.from_numpy(inds).to(DEV), torch.from_numpy(w).to(DEV)
+    seen = np.where(inds == 0, -1, inds)
+    xd = x.double().cpu().numpy()
+    y = K.switch_glu(L.g, L.slab.buf, table, experts, x, t)
+    ref, b = L.seam(xd, seen)
+    check(y, ref, b)
+    gone = torch.from_numpy((seen < 0) | (seen >= experts))
+    assert (y.cpu()[gone].view(torch.int16) == 0).all()
+    args = (L.g, L.slab.buf, table, experts)
+    out = K.moe_experts(*args, x, t, wt, L.shared_slot, gate)
+    ref, b = combined(L, xd, seen, w.astype(np.float64), gate.double().cpu().numpy())
+    check(out, ref, b)
+    if n <= 7:
+        for i in range(n):
+            r = slice(i, i + 1)
+            assert torch.equal(out[r], K.moe_experts(*args, x[r], t[r], wt[r], L.shared_slot, gate))
+            assert torch.equal(y[r], K.switch_glu(*args, x[r], t[r]))
+
+
 @pytest.mark.parametrize("gap", [1, 2, 4, 8])
 @pytest.mark.parametrize("n,pin", [(1, "0"), (20, "0"), (300, "0"), (300, "1")])
 def test_scales_anywhere(monkeypatch, n, pin, gap):

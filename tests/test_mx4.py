@@ -122,6 +122,16 @@ def test_expert_entries_refuse_rows_off_16_bytes(which):
     assert b"16 bytes" in L.pmoe_last_error()
 
 
+@pytest.mark.parametrize("hidden,inter,k,shared,experts", [
+    (32, 32, 1, 0, 1), (1024, 512, 4, 0, 32), (2048, 512, 10, 1, 512), (4096, 1536, 8, 0, 128),
+    (7168, 2048, 8, 1, 384), (32, 8192, 64, 0, 64), (64, 8192, 2, 1, 1000)])
+def test_workspace_of_a_call_serves_shorter_ones(hidden, inter, k, shared, experts):
+    L = _lib.lib()
+    g = _lib.geom(hidden, inter, 4, 32)
+    need = [L.pmoe_moe_workspace(ctypes.byref(g), n, k, shared, experts) for n in range(1, 80)]
+    assert need == sorted(need)
+
+
 def test_expert_entries_refuse_a_small_workspace():
     L = _lib.lib()
     g = _lib.geom(1024, 512, 4, 32)
