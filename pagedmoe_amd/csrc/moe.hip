@@ -99,7 +99,7 @@ size_t carve(const pmoe_geom* g, int n, int k, int shared, int n_experts, void* 
     t.hscale = c.take<uint8_t>(rows * mx_scale_row(g->inter));
     t.y = reinterpret_cast<float*>(c.take<uint16_t>(rows * g->hidden));
     // (also in longer calls' workspaces, which serve shorter calls)
-    const int one = std::min(n, mx_one_tokens(g, k, shared ? 1 : 0, n_experts, true));
+    const int one = mx_one_tokens(g, n, k, shared ? 1 : 0, n_experts, true);
     t.h32 = c.take<float>(size_t(one) * kk * g->inter);
     t.yscale = c.take<uint8_t>(rows * (g->hidden / kMxGroup));
   } else {

@@ -64,8 +64,9 @@ int mx_min_tile_rows();
 int mx_experts(const MxPlan& p, hipStream_t st);
 // Tokens one by one in two launches, without a dispatch: out bf16 [n, hidden]
 // combined (wts given) or [n, k, hidden].  slots [n, k + 1], h fp32 [n, k + 1, inter]:
-// scratch.  mx_one_tokens: the most tokens that go this way (the scratch's size).
-int mx_one_tokens(const pmoe_geom* g, int k, int shared, int n_experts, bool combined);
+// scratch.  mx_one_tokens: how many of n tokens may go this way (all of them or none do;
+// the scratch serves shorter calls too).
+int mx_one_tokens(const pmoe_geom* g, int n, int k, int shared, int n_experts, bool combined);
 bool mx_one_wanted(const pmoe_geom* g, int n, int k, int shared, int n_experts, bool combined);
 int mx_one(const pmoe_geom* g, const uint8_t* slab, const int32_t* table, int n_experts,
            const uint16_t* x, const int32_t* ids, const float* wts, int n, int k, int shared_slot,

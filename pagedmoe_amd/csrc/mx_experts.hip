@@ -1453,7 +1453,7 @@ int mx_experts(const MxPlan& p, hipStream_t st) {
                : launch_stream<false, false>(a, p.max_tiles, once, whole, st);
 }
 
-// The most tokens that go one by one (0: none may), in two launches instead of a
+// How many of n tokens may go one by one (0: none), in two launches instead of a
 // dispatch, the tiles' two and a combine.  What that saves, some 7 us and the combine,
 // pays for the weights that several of the tokens read (by expectation over
 // independent ids, and the shared expert's), and for a stream that is a tenth slower
@@ -1465,25 +1465,26 @@ int mx_experts(const MxPlan& p, hipStream_t st) {
 //     seam                            2: 40.2 / 38.5, 3: 53.3 / 53.8
 //   7168x2048 384 experts, 8 + shared 2: 91.7 / 94.0; seam, 8: 79.1 / 80.2
 // Up to 64 columns: a lane looks one up.
-int mx_one_tokens(const pmoe_geom* g, int k, int shared, int n_experts, bool combined) {
+int mx_one_tokens(const pmoe_geom* g, int n, int k, int shared, int n_experts, bool combined) {
   if (k + shared > 64) return 0;
+  if (n <= 1) return n;
   const double bytes = double(g->hidden) * g->inter / kMxGroup * 17 * 3;
   const double most = double((combined ? 36 : 24) << 20) / bytes;  // in experts
   const double absent = pow(1.0 - 1.0 / n_experts, k);  // an expert of one token's
   double none = absent;
-  int n = 1;
-  for (; n < 64; ++n) {  // would n + 1 do?
+  int t = 1;
+  for (; t < n && t < 64; ++t) {  // would t + 1 do?
     none *= absent;
     const double repeated =
-        double(n + 1) * k - n_experts * (1.0 - none) + double(shared) * n;
-    if (repeated + 0.1 * (n + 1) * (k + shared) > most) break;
+        double(t + 1) * k - n_experts * (1.0 - none) + double(shared) * t;
+    if (repeated + 0.1 * (t + 1) * (k + shared) > most) break;
   }
-  return n;
+  return t;
 }
 
 bool mx_one_wanted(const pmoe_geom* g, int n, int k, int shared, int n_experts, bool combined) {
   if (n > 1 && mx_pinned_rows()) return false;
-  return n <= mx_one_tokens(g, k, shared, n_experts, combined);
+  return n <= mx_one_tokens(g, n, k, shared, n_experts, combined);
 }
 
 int mx_one(const pmoe_geom* g, const uint8_t* slab, const int32_t* table, int n_experts,
