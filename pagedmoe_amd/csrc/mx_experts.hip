@@ -186,8 +186,8 @@ struct MxSplit {
 // A token by 256 threads, a lane a group: its pieces, scales and the mask of the
 // 128-wide steps that hold a third piece (16 bits a wave), the shared expert's gate
 // logit, the zero rows of ids that are dropped.  s_sum: 4 floats of the token's.
-// 16384 x 4096: 134 MB in, 280 MB out, 64 us beside the dispatch's scan.  Splitting in the products instead
-// would repeat these ~20 operations a value for every block of features.
+// 16384 x 4096: 134 MB in, 280 MB out, 64 us beside the dispatch's scan.  Splitting
+// in the products instead would repeat these ~20 operations a value for every block of features.
 __device__ __forceinline__ void split_token(const MxSplit& a, int token, int g, float* s_sum) {
   bool peak = false;
   float dot = 0.0f;
